@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define THA4_ABI_VERSION 6
+#define THA4_ABI_VERSION 7
 
 typedef enum tha4_status {
   THA4_OK = 0,
@@ -296,6 +296,90 @@ int tha4_display_rgba8(const float* frames_dev, int batch, int height, int width
  * RGBA8 image already on the device: /255 -> sRGB->linear on RGB -> premultiply alpha -> *2-1 -> HWC->CHW.
  * rgba_dev uint8 [B,H,W,4] -> out_dev fp32 [B,4,H,W]. */
 int tha4_ingest_rgba8(const uint8_t* rgba_dev, int batch, int height, int width, float* out_dev, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Operators of a transformer block over token sequences (ABI v7; no reference counterpart: the reference has attention, normalisation +
+ * FiLM + residual and matrix products only inside its fixed networks, src/tha4/nn/common/unet.py:90-97,157-163,192-239).  Stateless, device
+ * pointers of ONE GPU (which need not be the calling thread's current one), all work enqueued on `stream`; nothing allocates or synchronises, so
+ * every call can be captured into a graph.  A workspace belongs to one call in flight: two streams, or two captured graphs that may run
+ * at once, need one each.  Rows are `cols` contiguous elements, row_stride elements apart.  Outputs must not overlap inputs.
+ * Sizes of zero are valid (nothing is written) except where a sum would run over nothing (k, cols, head_dim).
+ * ------------------------------------------------------------------------------------------------ */
+typedef enum tha4_dtype { THA4_F32 = 0, THA4_F16 = 1, THA4_BF16 = 2 } tha4_dtype;
+
+/* q[r][c] = x[r][c] / scale[r] rounded to the nearest integer (ties to even, of the exact quotient), scale[r] = max_c |x[r][c]| / 127 in fp32.
+ * A row of zeros gets scale 0; a row that holds an infinity or a NaN gets scale NaN and zeros, so that products with it are NaN. */
+int tha4_quantize_tokens_i8(const void* x_dev, int x_dtype, int64_t rows, int64_t cols, int64_t x_row_stride, int8_t* q_dev, int64_t q_row_stride,
+                            float* scale_dev, void* stream);
+
+/* y[i][j] = x_scale[i] w_scale[j] sum_k x[i][k] w[j][k] + bias[j]: int8 x int8 with exact int32 sums (k <= 131071), scaled in fp32 and rounded once
+ * to y_dtype.  Any strides and alignments are valid; rows that are 16-byte aligned take the fast path. */
+typedef struct tha4_linear_i8_args {
+  const int8_t* x_dev;          /* [m][k] */
+  const float* x_scale_dev;     /* [m]    */
+  const int8_t* w_dev;          /* [n][k] */
+  const float* w_scale_dev;     /* [n]    */
+  const float* bias_dev;        /* [n] or NULL */
+  void* y_dev;                  /* [m][n] */
+  int64_t m, n, k;
+  int64_t x_row_stride, w_row_stride, y_row_stride;
+  int32_t y_dtype;
+} tha4_linear_i8_args;
+int tha4_linear_i8(const tha4_linear_i8_args* args, void* stream);
+
+/* The norms behind and in front of a block, with the gate and the residual sum between them:
+ *   h = residual_scale * residual_scale_vector * residual + gate * (post_norm(branch) * post_weight + post_bias)
+ *   y = (pre_norm(h) * pre_weight + pre_bias) * (1 + film_scale) + film_shift
+ * A norm is rms (v / sqrt(mean(v^2) + eps)) or layer (the same of v - mean(v)) over the `cols` elements of a row, or none; statistics in fp32, y from
+ * the unrounded h.  branch NULL: h = the scaled residual only.  h_dev NULL: h is not written; y_dev NULL: y is not computed.
+ * Row r reads gate row r / gate_rows and FiLM row r / film_rows (1 = a row for each token, tokens of a sample = a row for each sample, INT64_MAX = one).
+ * Vectors of `cols` are params_dtype: fp32, or dtype.  residual and h are residual_dtype: fp32, or dtype. */
+#define THA4_NORM_NONE 0
+#define THA4_NORM_RMS 1
+#define THA4_NORM_LAYER 2
+#define THA4_GATE_LINEAR 0
+#define THA4_GATE_SIGMOID 1
+typedef struct tha4_residual_norm_args {
+  const void *residual_dev, *branch_dev, *gate_dev;
+  const void *residual_scale_vector_dev, *post_weight_dev, *post_bias_dev, *pre_weight_dev, *pre_bias_dev; /* [cols] or NULL */
+  const void *film_scale_dev, *film_shift_dev;  /* params_dtype [rows / film_rows][cols], both or neither */
+  void *h_dev, *y_dev;
+  int64_t rows, cols;
+  int64_t residual_row_stride, branch_row_stride, gate_row_stride, film_row_stride, h_row_stride, y_row_stride;
+  int64_t gate_rows, film_rows;
+  int32_t dtype, residual_dtype, gate_dtype, params_dtype;   /* dtype: branch and y; gate_dtype: fp32, or dtype */
+  int32_t post_norm, pre_norm, gate_activation;
+  float residual_scale, eps;
+} tha4_residual_norm_args;
+int tha4_residual_norm(const tha4_residual_norm_args* args, void* stream);
+
+/* Differential attention: o = softmax(s q1 k1^T) v - lambda softmax(s q2 k2^T) v with lambda = exp(l0 . l1) - exp(l2 . l3) + lambda_init for each head
+ * (lambda_vectors [4][heads or 1][head_dim] fp32, in fp32), then, with `norm` non-zero, (1 - lambda_init) * o / sqrt(mean(o^2) + eps) * norm_weight.
+ *   q [batch][q_len][2 heads][d], k [batch][k_len][2 kv_heads][d]: heads 2h and 2h + 1 are the pair of head h;  v [batch][k_len][kv_heads][2d];
+ *   out [batch][q_len][heads][2d];  d = 32, 64 or 128;  heads a multiple of kv_heads;  dtype f16 or bf16; rows contiguous and 16-byte aligned;
+ *   strides in elements over (batch, token, head), token strides of k and v below 2^24.
+ * kv_lengths [batch] (NULL: k_len): keys at or behind it are never read into a result, whatever they hold.  q_lengths [batch] (NULL: q_len): query rows at or behind it are
+ * not written.  Lengths outside [0, k_len] / [0, q_len] count as the nearer end.  causal: query i sees key j <= i + kv_length - q_length (the last
+ * query the last key).  mask (NULL: none): bytes, non-zero = visible, over (batch, head, query, key) with strides in bytes (0 = broadcast).
+ * A query that sees no key answers zero.  A value that a query does not see does not reach its answer, infinities and NaN included.
+ * workspace_dev: tha4_diff_attention_workspace() bytes, 16-byte aligned (NULL if 0). */
+typedef struct tha4_diff_attention_args {
+  const void *q_dev, *k_dev, *v_dev;
+  void* out_dev;
+  const float* lambda_vectors_dev;
+  const float* norm_weight_dev;     /* [2d] fp32 or NULL (ones) */
+  const int32_t *q_lengths_dev, *kv_lengths_dev;
+  const uint8_t* mask_dev;
+  void* workspace_dev;
+  int64_t workspace_bytes;
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3], mask_stride[4];
+  int64_t lambda_vector_stride, lambda_head_stride;
+  int32_t dtype, batch, q_len, k_len, heads, kv_heads, head_dim;
+  int32_t causal, norm;
+  float scale, lambda_init, eps;
+} tha4_diff_attention_args;
+int64_t tha4_diff_attention_workspace(const tha4_diff_attention_args* args);
+int tha4_diff_attention(const tha4_diff_attention_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -4,6 +4,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
@@ -14,7 +15,10 @@ RESOURCES = os.path.join(CSRC, "libtha4_hip.resources.txt")
 # that differs from the shipped library is a memory-ordering / hazard fault in one of them (how round 3 found the faulty level-2
 # geometry).  TEST ARTEFACT: only tests/test_twin_gpu.py and tools/compare_libs.py load it, through THA4_HIP_LIB.
 TWIN = os.path.join(CSRC, "libtha4_hip_wait0.so")
-SOURCES = ["tha4_capi.hip"]
+# One object per source (kept under csrc/build/), so that a change to one family of kernels does not recompile the others (the posers' take minutes).
+# The order is the link order: the posers' code object is the first of the library.
+SOURCES = ["tha4_capi.hip", "tha4_transformer.hip"]
+OBJECTS = os.path.join(CSRC, "build")
 # No packed-fp32 VALU instructions (v_pk_mul / v_pk_fma / v_pk_add_f32) in any kernel of the library: the compiler's packed arithmetic is
 # what made level2_16p_kernel<8,.,2> produce run-to-run varying pixels on gfx950 once the sine shrank to one instruction
 # (profiles/r03_sin_cliff.md: wait states in front of every v_pk_* all but cure it, a build without them equals its forced-wait twin
@@ -22,8 +26,16 @@ SOURCES = ["tha4_capi.hip"]
 DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-DTHA4_NO_PACKED_FP32=1"]
 
 
-def _headers():
-    return sorted(f for f in os.listdir(CSRC) if f.endswith(".h"))
+def is_transformer_header(name: str) -> bool:
+    return name.startswith("transformer_")
+
+
+def _dependencies(source: str):
+    """Headers a source includes: transformer_*.h belong to tha4_transformer.hip alone, which includes nothing of the posers' kernels."""
+    own = source == "tha4_transformer.hip"
+    shared = ("tha4_platform.h", "tha4_tuning.h", "tha4_host.h")
+    heads = [f for f in sorted(os.listdir(CSRC)) if f.endswith(".h") and (f in shared or is_transformer_header(f) == own)]
+    return [os.path.join(CSRC, f) for f in [source] + heads] + [os.path.join(INCLUDE, "tha4_hip.h"), os.path.abspath(__file__)]
 
 
 def _stale(target: str, deps) -> bool:
@@ -40,31 +52,58 @@ def hipcc_path() -> str:
     return p
 
 
-def build_native(force: bool = False, verbose: bool = False) -> str:
-    deps = [os.path.join(CSRC, f) for f in SOURCES + _headers()] + [os.path.join(INCLUDE, "tha4_hip.h"), os.path.abspath(__file__)]
-    if not force and not _stale(LIB, deps) and os.path.exists(RESOURCES):
-        return LIB
-    cmd = [hipcc_path(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-Rpass-analysis=kernel-resource-usage"] + DEVICE_FLAGS + \
-          ["-I", CSRC, "-I", INCLUDE] + [os.path.join(CSRC, s) for s in SOURCES] + ["-o", LIB]
+def _compile(source: str, tag: str, extra, force: bool, verbose: bool = False) -> str:
+    """One source -> csrc/build/<name>.<tag>.o, with the resource report of its kernels beside it."""
+    os.makedirs(OBJECTS, exist_ok=True)
+    obj = os.path.join(OBJECTS, f"{os.path.splitext(source)[0]}.{tag}.o")
+    report = obj[:-2] + ".resources.txt"
+    if not force and not _stale(obj, _dependencies(source)) and os.path.exists(report):
+        return obj
+    cmd = [hipcc_path(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-c", "-Rpass-analysis=kernel-resource-usage"] + extra + DEVICE_FLAGS + \
+          ["-I", CSRC, "-I", INCLUDE, os.path.join(CSRC, source), "-o", obj]
     if verbose:
         print(" ".join(cmd))
     r = subprocess.run(cmd, stderr=subprocess.PIPE, text=True)
     if r.returncode != 0:
         raise RuntimeError("hipcc failed:\n" + r.stderr[-4000:])
-    with open(RESOURCES, "w") as f:          # per-kernel VGPR / scratch / LDS report (tests/test_api_surface.py gates on it)
+    with open(report, "w") as f:             # per-kernel VGPR / scratch / LDS report (tests/test_api_surface.py gates on it)
         f.write(parse_resource_remarks(r.stderr))
+    return obj
+
+
+def _link(target: str, tag: str, extra, force: bool, verbose: bool = False):
+    with ThreadPoolExecutor(len(SOURCES)) as pool:
+        objs = list(pool.map(lambda s: _compile(s, tag, extra, force, verbose), SOURCES))
+    if force or _stale(target, objs):
+        r = subprocess.run([hipcc_path(), "--offload-arch=gfx950", "-fPIC", "-shared"] + objs + ["-o", target], stderr=subprocess.PIPE, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("hipcc failed (link):\n" + r.stderr[-4000:])
+    return objs
+
+
+def _current(target: str, tag: str) -> bool:
+    """Whether the library is newer than every source and holds no object that is older than its own (a source edited while the others compiled)."""
+    for s in SOURCES:
+        obj = os.path.join(OBJECTS, f"{os.path.splitext(s)[0]}.{tag}.o")
+        if _stale(target, _dependencies(s)) or (os.path.exists(obj) and _stale(obj, _dependencies(s))):
+            return False
+    return True
+
+
+def build_native(force: bool = False, verbose: bool = False) -> str:
+    if not force and _current(LIB, "product") and os.path.exists(RESOURCES):
+        return LIB
+    objs = _link(LIB, "product", [], force, verbose)
+    with open(RESOURCES, "w") as f:
+        for o in objs:
+            f.write(open(o[:-2] + ".resources.txt").read())
     return LIB
 
 
 def build_forced_wait_twin(force: bool = False) -> str:
-    deps = [os.path.join(CSRC, f) for f in SOURCES + _headers()] + [os.path.join(INCLUDE, "tha4_hip.h"), os.path.abspath(__file__)]
-    if not force and not _stale(TWIN, deps):
+    if not force and _current(TWIN, "wait0"):
         return TWIN
-    cmd = [hipcc_path(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-mllvm", "-amdgpu-waitcnt-forcezero=1"] + DEVICE_FLAGS + \
-          ["-I", CSRC, "-I", INCLUDE] + [os.path.join(CSRC, s) for s in SOURCES] + ["-o", TWIN]
-    r = subprocess.run(cmd, stderr=subprocess.PIPE, text=True)
-    if r.returncode != 0:
-        raise RuntimeError("hipcc failed (forced-wait twin):\n" + r.stderr[-4000:])
+    _link(TWIN, "wait0", ["-mllvm", "-amdgpu-waitcnt-forcezero=1"], force)
     return TWIN
 
 

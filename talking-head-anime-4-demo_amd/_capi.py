@@ -15,7 +15,7 @@ import numpy as np
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "csrc", "libtha4_hip.so")
 
-THA4_ABI_VERSION = 6
+THA4_ABI_VERSION = 7
 STUDENT_EXACT_FP32 = 1
 FULL_EXACT_FP32 = 1
 FULL_EXACT_DECOMPOSER = 2
@@ -50,6 +50,34 @@ class Tha4StudentAux(C.Structure):
 
 
 ERR_NUMERIC_RANGE = -5
+
+# ---- operators of a transformer block (tha4_amd.transformer) ----
+F32, F16, BF16 = 0, 1, 2
+NORM_KINDS = {"none": 0, "rms": 1, "layer": 2}
+GATE_ACTIVATIONS = {"none": 0, "sigmoid": 1}
+
+
+class Tha4LinearI8Args(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x_dev", "x_scale_dev", "w_dev", "w_scale_dev", "bias_dev", "y_dev")] + \
+               [(n, C.c_int64) for n in ("m", "n", "k", "x_row_stride", "w_row_stride", "y_row_stride")] + [("y_dtype", C.c_int32)]
+
+
+class Tha4ResidualNormArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("residual_dev", "branch_dev", "gate_dev", "residual_scale_vector_dev", "post_weight_dev", "post_bias_dev",
+                                          "pre_weight_dev", "pre_bias_dev", "film_scale_dev", "film_shift_dev", "h_dev", "y_dev")] + \
+               [(n, C.c_int64) for n in ("rows", "cols", "residual_row_stride", "branch_row_stride", "gate_row_stride", "film_row_stride", "h_row_stride",
+                                         "y_row_stride", "gate_rows", "film_rows")] + \
+               [(n, C.c_int32) for n in ("dtype", "residual_dtype", "gate_dtype", "params_dtype", "post_norm", "pre_norm", "gate_activation")] + \
+               [("residual_scale", C.c_float), ("eps", C.c_float)]
+
+
+class Tha4DiffAttentionArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q_dev", "k_dev", "v_dev", "out_dev", "lambda_vectors_dev", "norm_weight_dev", "q_lengths_dev", "kv_lengths_dev",
+                                          "mask_dev", "workspace_dev")] + [("workspace_bytes", C.c_int64)] + \
+               [(n, C.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + [("mask_stride", C.c_int64 * 4)] + \
+               [(n, C.c_int64) for n in ("lambda_vector_stride", "lambda_head_stride")] + \
+               [(n, C.c_int32) for n in ("dtype", "batch", "q_len", "k_len", "heads", "kv_heads", "head_dim", "causal", "norm")] + \
+               [(n, C.c_float) for n in ("scale", "lambda_init", "eps")]
 
 
 def make_display(rgba8_ptr: int, background_rgb):
@@ -230,6 +258,16 @@ def load_library(path: Optional[str] = None) -> C.CDLL:
     lib.tha4_display_rgba8.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, c_float_p, C.c_void_p, C.c_void_p]
     lib.tha4_ingest_rgba8.restype = C.c_int
     lib.tha4_ingest_rgba8.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]
+    lib.tha4_quantize_tokens_i8.restype = C.c_int
+    lib.tha4_quantize_tokens_i8.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]
+    lib.tha4_linear_i8.restype = C.c_int
+    lib.tha4_linear_i8.argtypes = [C.POINTER(Tha4LinearI8Args), C.c_void_p]
+    lib.tha4_residual_norm.restype = C.c_int
+    lib.tha4_residual_norm.argtypes = [C.POINTER(Tha4ResidualNormArgs), C.c_void_p]
+    lib.tha4_diff_attention_workspace.restype = C.c_int64
+    lib.tha4_diff_attention_workspace.argtypes = [C.POINTER(Tha4DiffAttentionArgs)]
+    lib.tha4_diff_attention.restype = C.c_int
+    lib.tha4_diff_attention.argtypes = [C.POINTER(Tha4DiffAttentionArgs), C.c_void_p]
     v = lib.tha4_abi_version()
     if v != THA4_ABI_VERSION:
         raise Tha4Error(f"libtha4_hip.so ABI version {v} != expected {THA4_ABI_VERSION}")
@@ -244,6 +282,7 @@ EXPORTED_SYMBOLS = [
     "tha4_full_create", "tha4_full_create_ex", "tha4_full_num_networks", "tha4_full_flags", "tha4_full_set_fault_policy", "tha4_full_set_timing", "tha4_full_num_ops", "tha4_full_op_info", "tha4_full_last_op_ms", "tha4_full_pose", "tha4_full_pose_ex", "tha4_full_numeric_status",
     "tha4_full_destroy", "tha4_full_max_batch",
     "tha4_display_rgba8", "tha4_ingest_rgba8",
+    "tha4_quantize_tokens_i8", "tha4_linear_i8", "tha4_residual_norm", "tha4_diff_attention_workspace", "tha4_diff_attention",
 ]
 
 

@@ -14,35 +14,24 @@
 #include "siren16_kernels.h"
 #include "full_net.h"
 #include "image_io_kernels.h"
+#include "tha4_host.h"
 
 using namespace tha4;
 
-namespace {
+// the thread's last error (tha4_host.h: every entry point of the library reports through it)
+namespace tha4 {
+static thread_local std::string g_last_error;
 
-thread_local std::string g_last_error;
-
-int fail(int code, const std::string& msg) {
-  g_last_error = msg;
+int fail(int code, const char* msg) noexcept {
+  try {
+    g_last_error = msg;
+  } catch (...) {             // no memory for the text: the code is what remains
+  }
   return code;
 }
+}  // namespace tha4
 
-#define HIP_TRY(expr)                                                                              \
-  do {                                                                                             \
-    hipError_t e_ = (expr);                                                                        \
-    if (e_ != hipSuccess)                                                                          \
-      return fail(THA4_ERR_HIP, std::string(#expr) + ": " + hipGetErrorString(e_));                \
-  } while (0)
-
-struct DeviceGuard {
-  int prev = -1;
-  bool switched = false;
-  explicit DeviceGuard(int dev) {
-    if (hipGetDevice(&prev) == hipSuccess && prev != dev) switched = (hipSetDevice(dev) == hipSuccess);
-  }
-  ~DeviceGuard() {
-    if (switched) (void)hipSetDevice(prev);
-  }
-};
+namespace {
 
 constexpr int kNumKernels = 5;
 
@@ -77,13 +66,6 @@ struct StreamOrder {
     done = nullptr;
   }
 };
-
-// device that owns a device pointer (-1: unknown) - the stateless image entry points have no handle to ask
-int device_of(const void* p) {
-  hipPointerAttribute_t a;
-  if (hipPointerGetAttributes(&a, p) != hipSuccess) { (void)hipGetLastError(); return -1; }
-  return a.device;
-}
 
 }  // namespace
 

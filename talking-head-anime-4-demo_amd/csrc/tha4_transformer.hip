@@ -1,0 +1,251 @@
+// C-ABI implementation (include/tha4_hip.h) of the transformer block operators for MI355X (gfx950): argument checks and launches.
+// The kernels live in transformer_{norm,linear,attention}_kernels.h.  Nothing here allocates, synchronises or keeps state between calls.
+#include "tha4_hip.h"
+
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <string>
+
+#include "tha4_host.h"
+#include "transformer_attention_kernels.h"
+#include "transformer_linear_kernels.h"
+#include "transformer_norm_kernels.h"
+
+using namespace tha4;
+using namespace tha4::xf;
+
+namespace {
+
+constexpr int64_t kMaxGrid = 0x7fffffff;
+
+int64_t size_of(int dtype) { return dtype == THA4_F32 ? 4 : 2; }
+bool known(int dtype) { return dtype == THA4_F32 || dtype == THA4_F16 || dtype == THA4_BF16; }
+bool aligned(const void* p, int64_t row_stride, int64_t size) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row_stride * size % 16 == 0; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// the GPU all the pointers (NULL ones aside) live on, or -1
+template <int N>
+int one_device(const void* const (&p)[N]) {
+  int dev = -1;
+  for (const void* x : p) {
+    if (!x) continue;
+    const int d = device_of(x);
+    if (d < 0 || (dev >= 0 && d != dev)) return -1;
+    dev = d;
+  }
+  return dev;
+}
+
+int bad(const char* msg) { return fail(THA4_ERR_INVALID_ARGUMENT, msg); }
+
+template <class K, class A>
+int launch(K kernel, int64_t grid, int64_t grid_y, int threads, const A& a, void* stream) {
+  if (grid > kMaxGrid || grid_y > 65535) return bad("too many rows for one launch");
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid, (unsigned)grid_y), dim3(threads), 0, static_cast<hipStream_t>(stream), a);
+  HIP_TRY(hipGetLastError());
+  return THA4_OK;
+}
+
+// ---- quantisation ----
+template <class T>
+int quantize(const QuantArgs& a, void* stream) {
+  if (a.cols % 8 || !aligned(a.x, a.x_stride, sizeof(T)) || reinterpret_cast<uintptr_t>(a.q) % 8 || a.q_stride % 8 || a.cols > 16384)
+    return launch(quantize_any_kernel<T>, a.rows, 1, 256, a, stream);
+  if (a.cols <= 512) return launch(quantize_kernel<T, 64, 1>, ceil_div(a.rows, 4), 1, 256, a, stream);
+  if (a.cols <= 2048) return launch(quantize_kernel<T, 256, 1>, a.rows, 1, 256, a, stream);
+  if (a.cols <= 4096) return launch(quantize_kernel<T, 256, 2>, a.rows, 1, 256, a, stream);
+  if (a.cols <= 8192) return launch(quantize_kernel<T, 256, 4>, a.rows, 1, 256, a, stream);
+  return launch(quantize_kernel<T, 1024, 2>, a.rows, 1, 1024, a, stream);
+}
+
+// ---- norms ----
+template <class T, class R>
+int norm(const NormArgs& a, bool vector, void* stream) {
+  if (!vector || a.cols > 16384) return launch(residual_norm_any_kernel<T, R>, a.rows, 1, 256, a, stream);
+  if (a.cols <= 512) return launch(residual_norm_kernel<T, R, 64, 1>, ceil_div(a.rows, 4), 1, 256, a, stream);
+  if (a.cols <= 2048) return launch(residual_norm_kernel<T, R, 256, 1>, a.rows, 1, 256, a, stream);
+  if (a.cols <= 4096) return launch(residual_norm_kernel<T, R, 256, 2>, a.rows, 1, 256, a, stream);
+  if (a.cols <= 8192) return launch(residual_norm_kernel<T, R, 256, 4>, a.rows, 1, 256, a, stream);
+  return launch(residual_norm_kernel<T, R, 1024, 2>, a.rows, 1, 1024, a, stream);
+}
+
+// ---- attention ----
+// How the keys are divided among workgroups when there are few queries.  A pure function of the sizes: the workspace query and the launch agree.
+struct Plan {
+  bool few;
+  int row_tiles, splits, chunk;
+};
+Plan plan_of(const tha4_diff_attention_args& a) {
+  Plan p{};
+  const int64_t rows = (int64_t)a.q_len * (a.heads / a.kv_heads);
+  p.few = rows <= kRows;
+  p.splits = 1;
+  p.chunk = a.k_len;
+  if (!p.few) return p;
+  p.row_tiles = (int)ceil_div(rows, kRows);
+  const int64_t wgs = (int64_t)a.batch * a.kv_heads * p.row_tiles;
+  const int64_t want = ceil_div(1024, wgs);
+  int64_t chunk = ceil_div(ceil_div(a.k_len, want), 128) * 128;
+  if (chunk < 512) chunk = 512;
+  p.splits = (int)ceil_div(a.k_len, chunk);
+  if (p.splits < 1) p.splits = 1;
+  p.chunk = (int)chunk;
+  return p;
+}
+int64_t part_floats(int d) { return d == 32 ? Few<32>::PART : d == 64 ? Few<64>::PART : Few<128>::PART; }
+
+const char* check_shape(const tha4_diff_attention_args& a) {
+  if (a.batch < 0 || a.q_len < 0 || a.k_len < 0 || a.heads < 1 || a.kv_heads < 1) return "batch / q_len / k_len must not be negative, heads / kv_heads must be positive";
+  if (a.heads % a.kv_heads) return "heads must be a multiple of kv_heads";
+  if (a.head_dim != 32 && a.head_dim != 64 && a.head_dim != 128) return "head_dim must be 32, 64 or 128";
+  if (a.dtype != THA4_F16 && a.dtype != THA4_BF16) return "dtype must be f16 or bf16";
+  if (a.q_len > (1 << 30) || a.k_len > (1 << 30)) return "q_len / k_len must be at most 2^30";
+  if ((int64_t)a.q_len * (a.heads / a.kv_heads) > kMaxGrid) return "too many queries for one launch";
+  return nullptr;
+}
+
+template <class T, int D>
+int attention(AttnArgs& a, const Plan& p, void* stream) {
+  if (!p.few) return launch(diff_prompt_kernel<T, D>, (int64_t)a.batch * a.heads * ceil_div(a.q_len, kQueries), 1, 512, a, stream);
+  const int64_t tiles = (int64_t)a.batch * a.kv_heads * p.row_tiles;
+  const int st = launch(diff_few_kernel<T, D>, tiles * p.splits, 1, 256, a, stream);
+  if (st != THA4_OK || p.splits == 1) return st;
+  return launch(diff_join_kernel<T, D>, tiles, 1, 64, a, stream);
+}
+template <class T>
+int attention(AttnArgs& a, int d, const Plan& p, void* stream) {
+  return d == 32 ? attention<T, 32>(a, p, stream) : d == 64 ? attention<T, 64>(a, p, stream) : attention<T, 128>(a, p, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int tha4_quantize_tokens_i8(const void* x_dev, int x_dtype, int64_t rows, int64_t cols, int64_t x_row_stride, int8_t* q_dev, int64_t q_row_stride,
+                            float* scale_dev, void* stream) {
+  if (!known(x_dtype)) return bad("x_dtype must be f32, f16 or bf16");
+  if (rows < 0 || cols < 1) return bad("rows must not be negative and cols must be positive");
+  if (rows == 0) return THA4_OK;
+  if (!x_dev || !q_dev || !scale_dev) return bad("x / q / scale must not be NULL");
+  if (x_row_stride < 0 || q_row_stride < cols) return bad("x_row_stride must not be negative and q_row_stride must be at least cols");
+  const int dev = one_device({x_dev, q_dev, scale_dev});
+  if (dev < 0) return bad("x / q / scale must be device pointers of one GPU");
+  DeviceGuard guard(dev);
+  const QuantArgs a{x_dev, q_dev, scale_dev, rows, cols, x_row_stride, q_row_stride};
+  return x_dtype == THA4_F32 ? quantize<float>(a, stream) : x_dtype == THA4_F16 ? quantize<f16>(a, stream) : quantize<bf16>(a, stream);
+}
+
+int tha4_linear_i8(const tha4_linear_i8_args* args, void* stream) {
+  if (!args) return bad("args must not be NULL");
+  const tha4_linear_i8_args& g = *args;
+  if (!known(g.y_dtype)) return bad("y_dtype must be f32, f16 or bf16");
+  if (g.m < 0 || g.n < 0 || g.k < 1) return bad("m / n must not be negative and k must be positive");
+  if (g.k > 131071) return bad("k must be at most 131071 (the sums are 32-bit integers)");
+  if (g.m == 0 || g.n == 0) return THA4_OK;
+  if (!g.x_dev || !g.x_scale_dev || !g.w_dev || !g.w_scale_dev || !g.y_dev) return bad("x / x_scale / w / w_scale / y must not be NULL");
+  if (g.x_row_stride < 0 || g.w_row_stride < 0 || g.y_row_stride < g.n) return bad("row strides must not be negative and y_row_stride must be at least n");
+  const int dev = one_device({g.x_dev, g.x_scale_dev, g.w_dev, g.w_scale_dev, g.bias_dev, g.y_dev});
+  if (dev < 0) return bad("x / x_scale / w / w_scale / bias / y must be device pointers of one GPU");
+  DeviceGuard guard(dev);
+  const LinearArgs a{g.x_dev, g.w_dev, g.x_scale_dev, g.w_scale_dev, g.bias_dev, g.y_dev, g.m, g.n, g.k, g.x_row_stride, g.w_row_stride, g.y_row_stride, g.y_dtype};
+  const bool al = g.k % 16 == 0 && aligned(g.x_dev, g.x_row_stride, 1) && aligned(g.w_dev, g.w_row_stride, 1);
+  if (g.m <= 64) {
+    const int64_t nb = ceil_div(g.n, 16);
+    if (g.m <= 16) return al ? launch(linear_few_kernel<1, true>, nb, 1, 512, a, stream) : launch(linear_few_kernel<1, false>, nb, 1, 512, a, stream);
+    return al ? launch(linear_few_kernel<4, true>, nb, 1, 512, a, stream) : launch(linear_few_kernel<4, false>, nb, 1, 512, a, stream);
+  }
+  const int64_t nb = ceil_div(g.n, 128), mb = ceil_div(g.m, 128);
+  return al ? launch(linear_tile_kernel<true>, nb, mb, 256, a, stream) : launch(linear_tile_kernel<false>, nb, mb, 256, a, stream);
+}
+
+int tha4_residual_norm(const tha4_residual_norm_args* args, void* stream) {
+  if (!args) return bad("args must not be NULL");
+  const tha4_residual_norm_args& g = *args;
+  if (!known(g.dtype)) return bad("dtype must be f32, f16 or bf16");
+  for (int t : {g.residual_dtype, g.gate_dtype, g.params_dtype})
+    if (t != THA4_F32 && t != g.dtype) return bad("residual_dtype / gate_dtype / params_dtype must be f32 or dtype");
+  for (int t : {g.post_norm, g.pre_norm})
+    if (t != THA4_NORM_NONE && t != THA4_NORM_RMS && t != THA4_NORM_LAYER) return bad("unknown norm");
+  if (g.gate_activation != THA4_GATE_LINEAR && g.gate_activation != THA4_GATE_SIGMOID) return bad("unknown gate activation");
+  if (g.rows < 0 || g.cols < 1) return bad("rows must not be negative and cols must be positive");
+  if (!(g.eps >= 0.0f) || !std::isfinite(g.residual_scale)) return bad("eps must not be negative and residual_scale must be finite");
+  if (!g.residual_dev && g.rows) return bad("residual must not be NULL");
+  if (!g.branch_dev && (g.gate_dev || g.post_weight_dev || g.post_bias_dev)) return bad("a gate or a post norm's weights need a branch");
+  if (!g.film_scale_dev != !g.film_shift_dev) return bad("film_scale and film_shift come together");
+  if (!g.y_dev && (g.film_scale_dev || g.pre_weight_dev || g.pre_bias_dev)) return bad("a pre norm's weights or FiLM need y");
+  if (!g.h_dev && !g.y_dev && g.rows) return bad("one of h and y must be given");
+  if (g.rows == 0) return THA4_OK;
+  if ((g.gate_dev && g.gate_rows < 1) || (g.film_scale_dev && g.film_rows < 1)) return bad("gate_rows / film_rows must be positive");
+  if (g.residual_row_stride < 0 || g.branch_row_stride < 0 || g.gate_row_stride < 0 || g.film_row_stride < 0) return bad("row strides must not be negative");
+  if ((g.h_dev && g.h_row_stride < g.cols) || (g.y_dev && g.y_row_stride < g.cols)) return bad("output row strides must be at least cols");
+  const int dev = one_device({g.residual_dev, g.branch_dev, g.gate_dev, g.residual_scale_vector_dev, g.post_weight_dev, g.post_bias_dev, g.pre_weight_dev,
+                              g.pre_bias_dev, g.film_scale_dev, g.film_shift_dev, g.h_dev, g.y_dev});
+  if (dev < 0) return bad("residual / branch / gate / weights / film / h / y must be device pointers of one GPU");
+  DeviceGuard guard(dev);
+  NormArgs a{g.residual_dev, g.branch_dev, g.gate_dev, g.residual_scale_vector_dev, g.post_weight_dev, g.post_bias_dev, g.pre_weight_dev, g.pre_bias_dev,
+             g.film_scale_dev, g.film_shift_dev, g.h_dev, g.y_dev, g.rows, g.cols, g.residual_row_stride, g.branch_row_stride, g.gate_row_stride, g.film_row_stride,
+             g.h_row_stride, g.y_row_stride, g.gate_rows, g.film_rows, g.gate_dtype == THA4_F32, g.params_dtype == THA4_F32, g.post_norm, g.pre_norm,
+             g.gate_activation == THA4_GATE_SIGMOID, g.residual_scale, g.eps, 1.0f / (float)g.cols};
+  const int64_t st = size_of(g.dtype), sr = size_of(g.residual_dtype), sg = size_of(g.gate_dtype), sp = size_of(g.params_dtype);
+  const bool vector = g.cols % 8 == 0 && aligned(g.residual_dev, g.residual_row_stride, sr) && aligned(g.branch_dev, g.branch_row_stride, st) &&
+                      aligned(g.gate_dev, g.gate_dev ? g.gate_row_stride : 0, sg) && aligned(g.film_scale_dev, g.film_scale_dev ? g.film_row_stride : 0, sp) &&
+                      aligned(g.film_shift_dev, 0, sp) && aligned(g.h_dev, g.h_dev ? g.h_row_stride : 0, sr) && aligned(g.y_dev, g.y_dev ? g.y_row_stride : 0, st) &&
+                      aligned(g.residual_scale_vector_dev, 0, sp) && aligned(g.post_weight_dev, 0, sp) && aligned(g.post_bias_dev, 0, sp) &&
+                      aligned(g.pre_weight_dev, 0, sp) && aligned(g.pre_bias_dev, 0, sp);
+  if (g.dtype == THA4_F32) return norm<float, float>(a, vector, stream);
+  if (g.dtype == THA4_F16) return g.residual_dtype == THA4_F32 ? norm<f16, float>(a, vector, stream) : norm<f16, f16>(a, vector, stream);
+  return g.residual_dtype == THA4_F32 ? norm<bf16, float>(a, vector, stream) : norm<bf16, bf16>(a, vector, stream);
+}
+
+int64_t tha4_diff_attention_workspace(const tha4_diff_attention_args* args) {
+  if (!args) return bad("args must not be NULL");
+  if (const char* e = check_shape(*args)) return bad(e);
+  const Plan p = plan_of(*args);
+  return p.splits == 1 ? 0 : (int64_t)args->batch * args->kv_heads * p.row_tiles * p.splits * part_floats(args->head_dim) * 4;
+}
+
+int tha4_diff_attention(const tha4_diff_attention_args* args, void* stream) {
+  if (!args) return bad("args must not be NULL");
+  const tha4_diff_attention_args& g = *args;
+  if (const char* e = check_shape(g)) return bad(e);
+  if (!(g.scale > 0.0f) || !std::isfinite(g.scale)) return bad("scale must be positive and finite");
+  if (!(g.eps >= 0.0f) || !std::isfinite(g.lambda_init)) return bad("eps must not be negative and lambda_init must be finite");
+  if (g.batch == 0 || g.q_len == 0) return THA4_OK;
+  if (!g.q_dev || !g.out_dev || !g.lambda_vectors_dev) return bad("q / out / lambda_vectors must not be NULL");
+  if (g.k_len && (!g.k_dev || !g.v_dev)) return bad("k / v must not be NULL");
+  if (reinterpret_cast<uintptr_t>(g.q_dev) % 16 || reinterpret_cast<uintptr_t>(g.k_dev) % 16 || reinterpret_cast<uintptr_t>(g.v_dev) % 16 || reinterpret_cast<uintptr_t>(g.out_dev) % 8)
+    return bad("q / k / v must be 16-byte aligned, out 8-byte");
+  for (int i = 0; i < 3; ++i) {
+    if (g.q_stride[i] % 8 || g.k_stride[i] % 8 || g.v_stride[i] % 8 || g.out_stride[i] % 4) return bad("strides of q / k / v must be multiples of 8 elements, of out of 4");
+    if (i == 1 && (g.k_stride[i] >= (1 << 24) || g.v_stride[i] >= (1 << 24))) return bad("token strides of k / v must be below 2^24 elements");
+    if (g.q_stride[i] < 0 || g.k_stride[i] < 0 || g.v_stride[i] < 0 || g.out_stride[i] < 0) return bad("strides must not be negative");
+  }
+  for (int i = 0; i < 4; ++i)
+    if (g.mask_dev && g.mask_stride[i] < 0) return bad("strides must not be negative");
+  if (g.lambda_vector_stride < 0 || g.lambda_head_stride < 0) return bad("strides must not be negative");
+  const Plan p = plan_of(g);
+  const int64_t need = tha4_diff_attention_workspace(args);
+  if (need && (!g.workspace_dev || g.workspace_bytes < need || reinterpret_cast<uintptr_t>(g.workspace_dev) % 16))
+    return bad("workspace is smaller than tha4_diff_attention_workspace() or not 16-byte aligned");
+  const int dev = one_device({g.q_dev, g.k_len ? g.k_dev : nullptr, g.k_len ? g.v_dev : nullptr, g.out_dev, g.lambda_vectors_dev, g.norm_weight_dev, g.q_lengths_dev,
+                              g.kv_lengths_dev, g.k_len ? g.mask_dev : nullptr, need ? g.workspace_dev : nullptr});
+  if (dev < 0) return bad("q / k / v / out / weights / lengths / mask / workspace must be device pointers of one GPU");
+  DeviceGuard guard(dev);
+  AttnArgs a{};
+  a.q = g.q_dev; a.k = g.k_dev; a.v = g.v_dev; a.out = g.out_dev;
+  a.lambdas = g.lambda_vectors_dev; a.norm_w = g.norm_weight_dev;
+  a.q_lengths = g.q_lengths_dev; a.kv_lengths = g.kv_lengths_dev;
+  a.mask = g.k_len ? g.mask_dev : nullptr;
+  a.work = static_cast<float*>(g.workspace_dev);
+  for (int i = 0; i < 3; ++i) { a.qs[i] = g.q_stride[i]; a.ks[i] = g.k_stride[i]; a.vs[i] = g.v_stride[i]; a.os[i] = g.out_stride[i]; }
+  for (int i = 0; i < 4; ++i) a.ms[i] = g.mask_stride[i];
+  a.lambda_vs = g.lambda_vector_stride; a.lambda_hs = g.lambda_head_stride;
+  a.batch = g.batch; a.q_len = g.q_len; a.k_len = g.k_len; a.heads = g.heads; a.kv_heads = g.kv_heads; a.group = g.heads / g.kv_heads;
+  a.causal = g.causal; a.norm = g.norm;
+  a.row_tiles = p.row_tiles; a.splits = p.splits; a.chunk = p.chunk;
+  a.c = g.scale * 1.44269504088896340736f; a.lambda_init = g.lambda_init; a.eps = g.eps;
+  return g.dtype == THA4_F16 ? attention<f16>(a, g.head_dim, p, stream) : attention<bf16>(a, g.head_dim, p, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,570 @@
+// Differential attention (tha4_diff_attention): for each head two softmax maps over the same keys and one value matrix of twice the width,
+//   o = softmax(s q1 k1^T) v - lambda softmax(s q2 k2^T) v,   out = (1 - lambda_init) o / sqrt(mean(o^2) + eps) w
+// One pass over the keys with the running maximum m and sum l of each map:  p = exp(s x - m), l = sum p, O = sum p v, out of which O / l.
+//
+// Every product is written transposed, with the queries along the matrix instruction's columns:  S^T = K Q^T and O^T = V^T P^T.  A lane then holds scores of ONE
+// query (column lane % 32 or lane % 16): maxima and sums are registers of the lane plus one exchange with the lanes of the same column, a
+// rescale is one multiplier a lane, and the accumulator layout of S^T is already an operand layout for P^T - which key sits in which k slot of the
+// product with V is free as long as V^T uses the same order, so P never leaves its registers.  V^T operands come from row-major V in LDS by the transposing read
+// ds_read_b64_tr_b16 (four keys of one column a lane).
+#pragma once
+#include "transformer_types.h"
+
+namespace tha4 {
+namespace xf {
+
+struct AttnArgs {
+  const void *q, *k, *v;
+  void* out;
+  const float *lambdas, *norm_w;
+  const int32_t *q_lengths, *kv_lengths;
+  const uint8_t* mask;
+  float* work;
+  int64_t qs[3], ks[3], vs[3], os[3], ms[4];
+  int64_t lambda_vs, lambda_hs;
+  int32_t batch, q_len, k_len, heads, kv_heads, group, causal, norm;
+  int32_t row_tiles, splits, chunk;
+  float c, lambda_init, eps;                   // c = scale * log2(e): the softmax is taken in powers of two
+};
+
+template <class T> struct Mat;
+template <> struct Mat<f16> {
+  typedef f16x8 v8;
+  static THA4_DEV f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+  static THA4_DEV f32x4 mma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mat<bf16> {
+  typedef bf16x8 v8;
+  static THA4_DEV f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+  static THA4_DEV f32x4 mma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+// lane i of each 16 receives column i of the 4 x 16 block of 16-bit values whose row r the lanes 4r .. 4r+3 address (8 bytes each)
+THA4_DEV s16x4 read_transposed(const char* lds) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds));
+}
+template <class V8>
+THA4_DEV V8 join(s16x4 a, s16x4 b) { return __builtin_bit_cast(V8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)); }
+
+THA4_DEV float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
+THA4_DEV float other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+struct Lengths { int q, k; };
+THA4_DEV Lengths lengths_of(const AttnArgs& a, int b) {
+  Lengths n;
+  n.q = a.q_lengths ? min(max(a.q_lengths[b], 0), a.q_len) : a.q_len;
+  n.k = a.kv_lengths ? min(max(a.kv_lengths[b], 0), a.k_len) : a.k_len;
+  return n;
+}
+// exp(l0 . l1) - exp(l2 . l3) + lambda_init of a head, by one wave
+template <int D>
+THA4_DEV float lambda_of(const AttnArgs& a, int head) {
+  const float* l = a.lambdas + head * a.lambda_hs;
+  float s = 0.0f, t = 0.0f;
+  for (int i = threadIdx.x & 63; i < D; i += 64) {
+    s = fmaf(l[i], l[a.lambda_vs + i], s);
+    t = fmaf(l[2 * a.lambda_vs + i], l[3 * a.lambda_vs + i], t);
+  }
+  return expf(wave_reduce(s, Add())) - expf(wave_reduce(t, Add())) + a.lambda_init;
+}
+
+// ---- prompts: many queries ---------------------------------------------------------------------------------------------------------------
+// A workgroup owns 128 queries of one head: eight waves, wave w the queries 32 (w % 4) .. + 31 of map w / 4 (the maps meet once, at the end: each wave carries one
+// map's accumulator, which is what lets 2 x 2d columns fit the registers).  Keys go through LDS in tiles of 64: K of both maps and V.
+// The 16-byte pieces of a K row are permuted so that the 16 lanes the LDS serves together read 16 different slots, those of a V row so that
+// the four rows of a transposing read lie in different quarters of the banks.
+constexpr int kKeys = 64, kQueries = 128;
+
+template <int D>
+struct Tile {
+  static constexpr int KP = D / 8, VP = D / 4;                         // 16-byte pieces of a K row (one map), of a V row
+  static constexpr int K_BYTES = 2 * kKeys * KP * 16, V_BYTES = kKeys * VP * 16, BYTES = K_BYTES + V_BYTES;
+  static THA4_DEV int k_swizzle(int row) { return (row / (16 / KP)) & (KP - 1); }
+  static THA4_DEV int v_swizzle(int row) { return VP == 8 ? ((row >> 1) & 1) * 4 : (row & 3) * 4; }
+};
+
+// Copies the tile of keys k0 .. k0 + 63 into LDS: per instruction a wave moves 64 pieces, 64 / KP rows of K or 64 / VP rows of V; keys behind the last repeat the last one.
+// kb, vb: the rows of key k0 (scalar); offsets inside a tile fit 32 bits (the host bounds the strides).
+template <class T, int D>
+THA4_DEV void load_tile(const AttnArgs& a, const T* kb, const T* vb, int left, char* lds) {
+  typedef Tile<D> L;
+  const int lane = threadIdx.x & 63, wave = uniform_i32(threadIdx.x >> 6);
+  constexpr int KR = 8 * 64 / L::KP, VR = 8 * 64 / L::VP;              // rows that the eight waves move per instruction
+  const unsigned ks = (unsigned)a.ks[1], vs = (unsigned)a.vs[1];
+  const int kw = wave * (KR / 8), krow = kw % kKeys + lane / L::KP;
+  const unsigned kcol = 8 * ((lane % L::KP) ^ L::k_swizzle(krow));     // (the swizzles repeat after 16 rows: the same for every instruction of the wave)
+  const int vrow = wave * (VR / 8) + lane / L::VP;
+  const unsigned vcol = 8 * ((lane % L::VP) ^ L::v_swizzle(vrow));
+#pragma unroll
+  for (int u = 0; u < L::K_BYTES / 8192; ++u)
+    glds16(kb + (u * KR / kKeys + kw / kKeys) * a.ks[2] + ((unsigned)min(krow + (u * KR) % kKeys, left) * ks + kcol), lds + (u * 8 + wave) * 1024);
+#pragma unroll
+  for (int u = 0; u < L::V_BYTES / 8192; ++u)
+    glds16(vb + ((unsigned)min(vrow + u * VR, left) * vs + vcol), lds + L::K_BYTES + (u * 8 + wave) * 1024);
+}
+
+// A tile of which some query sees only a part, with an infinity or a NaN in V: 0 * inf must not reach a query that does not see that key.  The value is added
+// to the accumulators that do see it, and taken out of the tile.  Rare: written for size.
+template <class T, int D>
+THA4_DEV void quarantine(const AttnArgs& a, char* vt, f32x16 (&acc)[D / 16], int k0, int limit, const uint8_t* mask, int* flag) {
+  typedef Tile<D> L;
+  const int lane = threadIdx.x & 63;
+  auto finite16 = [](unsigned short u) { return sizeof(T) && (std::is_same<T, bf16>::value ? (u & 0x7f80) != 0x7f80 : (u & 0x7c00) != 0x7c00); };
+  bool bad = false;
+  for (int p = threadIdx.x; p < L::V_BYTES / 2; p += 512) bad |= !finite16(reinterpret_cast<const unsigned short*>(vt)[p]);
+  if (bad) *flag = 1;
+  __syncthreads();
+  const bool any = *flag != 0;
+  __syncthreads();
+  if (!any) return;
+  for (int key = 0; key < kKeys; ++key) {
+    const bool seen = k0 + key < limit && (!mask || mask[(int64_t)(k0 + key) * a.ms[3]]);
+    const T* row = reinterpret_cast<const T*>(vt + key * L::VP * 16);
+    int h = lane >> 5;
+    asm volatile("" : "+v"(h));                                        // (addresses computed here, not kept from the loop's head: they would cost the main loop registers)
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int dv = 32 * t + 8 * (r / 4) + 4 * h + r % 4;
+        const T val = row[8 * ((dv / 8) ^ L::v_swizzle(key)) + dv % 8];
+        if (seen && !finite16(__builtin_bit_cast(unsigned short, val))) acc[t][r] += (float)val;
+      }
+      THA4_SCHED_FENCE();                                              // (a few values at a time: nothing here may cost the main loop registers)
+    }
+  }
+  __syncthreads();
+  for (int p = threadIdx.x; p < L::V_BYTES / 2; p += 512) {
+    unsigned short* u = reinterpret_cast<unsigned short*>(vt) + p;
+    if (!finite16(*u)) *u = 0;
+  }
+  if (threadIdx.x == 0) *flag = 0;
+  __syncthreads();
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(512, 2) diff_prompt_kernel(AttnArgs a) {
+  warm_kernarg<(int)sizeof(AttnArgs)>();
+  typedef Tile<D> L;
+  typedef typename Mat<T>::v8 v8;
+  constexpr int VT = D / 16;                                           // tiles of 32 value columns
+  constexpr int J = D == 128 ? 1 : 2;                                  // groups of 32 keys a softmax step takes: one where the accumulator leaves no registers for two
+  constexpr int JOIN = 4 * VT * 16 * 64 * 4;                           // bytes in which the second maps' results meet the first's
+  __shared__ __attribute__((aligned(16))) char lds[L::BYTES > JOIN ? L::BYTES : JOIN];
+  __shared__ int flag;
+  const int lane = threadIdx.x & 63, wave = uniform_i32(threadIdx.x >> 6), map = wave >> 2, h = lane >> 5;
+  const int bh = blockIdx.x % (a.batch * a.heads), b = bh / a.heads, head = bh % a.heads;
+  const int q0 = ((int)(gridDim.x / (a.batch * a.heads)) - 1 - (int)(blockIdx.x / (a.batch * a.heads))) * kQueries;     // the longest rows of a causal map first
+  const Lengths n = lengths_of(a, b);
+  if (q0 >= n.q) return;
+  if (threadIdx.x == 0) flag = 0;
+  const int kv = head / a.group, off = n.k - n.q;
+  const int qw = q0 + 32 * (wave & 3), qi = qw + (lane & 31), row = min(qi, n.q - 1);
+  const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + row * a.qs[1] + (2 * head + map) * a.qs[2];
+  const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + 2 * kv * a.ks[2];
+  const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2];
+  const uint8_t* mask = a.mask ? a.mask + b * a.ms[0] + head * a.ms[1] + row * a.ms[2] : nullptr;
+  v8 qf[D / 16];
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) qf[s] = *reinterpret_cast<const v8*>(q + 16 * s + 8 * h);
+  const int limit = a.causal ? min(n.k, row + off + 1) : n.k;          // this query sees keys below it
+  const int wg_end = a.causal ? min(n.k, min(q0 + kQueries, n.q) + off) : n.k;
+  const int wg_full = a.mask ? 0 : a.causal ? min(n.k, q0 + off + 1) : n.k;      // every query of the workgroup sees the keys below it
+  f32x16 acc[VT];
+#pragma unroll
+  for (int t = 0; t < VT; ++t) acc[t] = f32x16{0};
+  float m = -INFINITY, l = 0.0f;
+
+  auto tile = [&](int k0, auto part_) {
+    constexpr bool part = decltype(part_)::value;
+    __syncthreads();
+    load_tile<T, D>(a, k + (int64_t)k0 * a.ks[1], v + (int64_t)k0 * a.vs[1], n.k - 1 - k0, lds);
+    __syncthreads();
+    const char* kt = lds + map * (L::K_BYTES / 2);
+    char* vt = lds + L::K_BYTES;
+    if constexpr (part) quarantine<T, D>(a, vt, acc, k0, limit, mask, &flag);
+#pragma unroll
+    for (int j0 = 0; j0 < 2; j0 += J) {
+      f32x16 s[J];
+#pragma unroll
+      for (int i = 0; i < J; ++i) {
+        s[i] = f32x16{0};
+        const int r = 32 * (j0 + i) + (lane & 31);
+#pragma unroll
+        for (int u = 0; u < D / 16; ++u) {
+          const v8 kf = *reinterpret_cast<const v8*>(kt + (r * L::KP + ((2 * u + h) ^ L::k_swizzle(r))) * 16);
+          s[i] = Mat<T>::mma32(kf, qf[u], s[i]);
+        }
+      }
+      if constexpr (part) {
+#pragma unroll
+        for (int i = 0; i < J; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int key = k0 + 32 * (j0 + i) + 8 * (r / 4) + 4 * h + r % 4;
+            bool seen = key < limit;
+            if (mask) {
+              seen = seen && mask[(int64_t)min(key, a.k_len - 1) * a.ms[3]];
+              if (r % 4 == 3) THA4_SCHED_FENCE();
+            }
+            s[i][r] = seen ? s[i][r] : -INFINITY;
+          }
+      }
+      THA4_SCHED_FENCE();
+      float top = s[0][0];
+#pragma unroll
+      for (int i = 0; i < J; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
+      top = fmaxf(top, other_half(top));
+      if (__any(top > m)) {
+        const float now = fmaxf(m, top), w = now == -INFINITY ? 1.0f : exp2_((m - now) * a.c);
+        l *= w;
+#pragma unroll
+        for (int t = 0; t < VT; ++t) acc[t] *= w;
+        m = now;
+      }
+      const float mc = m == -INFINITY ? 0.0f : m * a.c;
+      v8 pf[2 * J];
+#pragma unroll
+      for (int i = 0; i < J; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float p = exp2_(fmaf(s[i][r], a.c, -mc));
+          l += p;
+          pf[2 * i + r / 8][r % 8] = (T)p;
+        }
+      THA4_SCHED_FENCE();
+      // k slot (h, e) of the product's step u holds key 16 u + 8 (e / 4) + 4 h + e % 4: the accumulator layout of S^T
+#pragma unroll
+      for (int u = 0; u < 2 * J; ++u)
+#pragma unroll
+        for (int t = 0; t < VT; ++t) {
+          const int r0 = 32 * j0 + 16 * u + 4 * h + ((lane & 15) >> 2), piece = 4 * t + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), in = 8 * (lane & 1);
+          const s16x4 lo = read_transposed(vt + (r0 * L::VP + (piece ^ L::v_swizzle(r0))) * 16 + in);
+          const s16x4 hi = read_transposed(vt + ((r0 + 8) * L::VP + (piece ^ L::v_swizzle(r0 + 8))) * 16 + in);
+          acc[t] = Mat<T>::mma32(join<v8>(lo, hi), pf[u], acc[t]);
+        }
+      THA4_SCHED_FENCE();
+    }
+  };
+  int k0 = 0;
+  for (; k0 + kKeys <= wg_full; k0 += kKeys) tile(k0, std::false_type());
+  for (; k0 < wg_end; k0 += kKeys) tile(k0, std::true_type());
+
+  l += other_half(l);
+  float* meet = reinterpret_cast<float*>(lds) + (wave & 3) * (VT * 16 * 64) + lane;
+  __syncthreads();
+  if (map == 1) {
+    const float lam = lambda_of<D>(a, head), w = l > 0.0f || l != l ? lam / l : 0.0f;      // (no key seen: nothing)
+#pragma unroll
+    for (int t = 0; t < VT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) meet[(t * 16 + r) * 64] = acc[t][r] * w;
+  }
+  __syncthreads();
+  if (map == 1) return;
+  const float w = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+  float ss = 0.0f;
+#pragma unroll
+  for (int t = 0; t < VT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      acc[t][r] = fmaf(acc[t][r], w, -meet[(t * 16 + r) * 64]);
+      ss = fmaf(acc[t][r], acc[t][r], ss);
+    }
+  ss += other_half(ss);
+  if (qi >= n.q) return;
+  const float g = a.norm ? (1.0f - a.lambda_init) / sqrtf(ss * (1.0f / (2 * D)) + a.eps) : 1.0f;
+  T* out = static_cast<T*>(a.out) + b * a.os[0] + qi * a.os[1] + head * a.os[2];
+  typedef T T4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int t = 0; t < VT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int dv = 32 * t + 8 * r + 4 * h;
+      T4 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = (T)(acc[t][4 * r + e] * g * (a.norm && a.norm_w ? a.norm_w[dv + e] : 1.0f));
+      *reinterpret_cast<T4*>(out + dv) = o;
+    }
+}
+
+// ---- few queries over a long cache -------------------------------------------------------------------------------------------------------
+// The cache is the traffic: 4 d elements a key and kv head, read once for all queries and heads that share it (up to 16 rows, the columns of the 16 x 16 x 32 products).
+// A workgroup owns a range of the keys; its four waves take turns of 32 keys, each with running statistics of its own and without barriers: K from memory into
+// operand registers, V through the wave's own LDS for the transposing read.  The waves meet in LDS, the ranges in a second launch.
+constexpr int kTurn = 32, kRows = 16;
+
+template <int D>
+struct Few {
+  static constexpr int VP = D / 4, VT = D / 8;                         // pieces of a V row; tiles of 16 value columns
+  static constexpr int V_BYTES = kTurn * VP * 16;                      // one wave's V
+  static constexpr int SET = 2 * VT * 4 * 64;                          // floats of one wave's (or range's) two accumulators
+  static constexpr int PART = SET + 4 * kRows;                         // ... and their statistics: m1, l1, m2, l2 of each row
+  static THA4_DEV int v_swizzle(int row) { return VP == 8 ? ((row >> 1) & 3) * 2 : (row & 7) * 2; }
+};
+
+// out of O1, l1, O2, l2 (accumulator layout: row lane % 16, value columns 16 t + 4 (lane / 16) + e)
+template <class T, int D>
+THA4_DEV void finish_few(const AttnArgs& a, f32x4 (&o)[2][D / 8], float l1, float l2, int b, int kv, int R, int rows, int q_valid) {
+  const int lane = threadIdx.x & 63, head = kv * a.group + R % a.group, qi = R / a.group;
+  // (every lane of the wave takes part in the sums of lambda: the heads of a wave's rows differ)
+  const float* l = a.lambdas + min(head, a.heads - 1) * a.lambda_hs;
+  float s = 0.0f, t2 = 0.0f;
+  for (int i = lane >> 4; i < D; i += 4) {
+    s = fmaf(l[i], l[a.lambda_vs + i], s);
+    t2 = fmaf(l[2 * a.lambda_vs + i], l[3 * a.lambda_vs + i], t2);
+  }
+  s += __shfl_xor(s, 16, 64); s += __shfl_xor(s, 32, 64);
+  t2 += __shfl_xor(t2, 16, 64); t2 += __shfl_xor(t2, 32, 64);
+  const float lam = expf(s) - expf(t2) + a.lambda_init;
+  const float w1 = l1 > 0.0f || l1 != l1 ? 1.0f / l1 : 0.0f, w2 = l2 > 0.0f || l2 != l2 ? lam / l2 : 0.0f;
+  float ss = 0.0f;
+#pragma unroll
+  for (int t = 0; t < D / 8; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o[0][t][e] = o[0][t][e] * w1 - o[1][t][e] * w2;
+      ss = fmaf(o[0][t][e], o[0][t][e], ss);
+    }
+  ss += __shfl_xor(ss, 16, 64);
+  ss += __shfl_xor(ss, 32, 64);
+  if (R >= rows || qi >= q_valid) return;
+  const float g = a.norm ? (1.0f - a.lambda_init) / sqrtf(ss * (1.0f / (2 * D)) + a.eps) : 1.0f;
+  T* out = static_cast<T*>(a.out) + b * a.os[0] + qi * a.os[1] + head * a.os[2];
+  typedef T T4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+  for (int t = 0; t < D / 8; ++t) {
+    const int dv = 16 * t + 4 * (lane >> 4);
+    T4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r[e] = (T)(o[0][t][e] * g * (a.norm && a.norm_w ? a.norm_w[dv + e] : 1.0f));
+    *reinterpret_cast<T4*>(out + dv) = r;
+  }
+}
+
+template <class T, int D>
+__global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArgs a) {
+  warm_kernarg<(int)sizeof(AttnArgs)>();
+  typedef Few<D> L;
+  typedef typename Mat<T>::v8 v8;
+  constexpr int LDS = 4 * L::V_BYTES > 2 * L::SET * 4 ? 4 * L::V_BYTES : 2 * L::SET * 4;
+  __shared__ __attribute__((aligned(16))) char lds[LDS];
+  __shared__ float stat[4][4][kRows];
+  const int lane = threadIdx.x & 63, wave = uniform_i32(threadIdx.x >> 6), g = lane >> 4;
+  int id = blockIdx.x;
+  const int split = id % a.splits; id /= a.splits;
+  const int rt = id % a.row_tiles; id /= a.row_tiles;
+  const int kv = id % a.kv_heads, b = id / a.kv_heads;
+  const Lengths n = lengths_of(a, b);
+  const int rows = a.q_len * a.group, R = rt * kRows + (lane & 15), Rc = min(R, rows - 1);
+  const int qi = min(Rc / a.group, max(n.q - 1, 0)), head = kv * a.group + Rc % a.group;
+  const int begin = split * a.chunk, end = min(n.k, begin + a.chunk);
+  if (a.splits > 1 && begin >= n.k) return;                              // (the join knows the length too)
+  const int limit = a.causal ? min(n.k, qi + (n.k - n.q) + 1) : n.k;
+  const int q_first = (rt * kRows) / a.group;
+  const int full = a.mask ? 0 : a.causal ? min(n.k, q_first + (n.k - n.q) + 1) : n.k;
+  const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + qi * a.qs[1] + 2 * head * a.qs[2];
+  const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + 2 * kv * a.ks[2];
+  const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2];
+  const uint8_t* mask = a.mask ? a.mask + b * a.ms[0] + head * a.ms[1] + qi * a.ms[2] : nullptr;
+  v8 qf[2][D / 32];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int u = 0; u < D / 32; ++u) qf[i][u] = *reinterpret_cast<const v8*>(q + i * a.qs[2] + 32 * u + 8 * g);
+  f32x4 acc[2][L::VT];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int t = 0; t < L::VT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  char* vt = lds + wave * L::V_BYTES;
+
+  for (int k0 = begin + wave * kTurn; k0 < end; k0 += 4 * kTurn) {
+    const int last = n.k - 1;
+    v8 kf[2][2][D / 32];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const T* kr = k + (int64_t)min(k0 + 16 * j + (lane & 15), last) * a.ks[1] + 8 * g;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int u = 0; u < D / 32; ++u) kf[i][j][u] = *reinterpret_cast<const v8*>(kr + i * a.ks[2] + 32 * u);
+    }
+#pragma unroll
+    for (int u = 0; u < L::V_BYTES / 1024; ++u) {
+      const int p = u * 64 + lane, row = p / L::VP, pos = p % L::VP;
+      glds16(v + (int64_t)min(k0 + row, last) * a.vs[1] + 8 * (pos ^ L::v_swizzle(row)), vt + u * 1024);
+    }
+    v8 pf[2];
+    const bool part = k0 + kTurn > full;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      f32x4 s[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        s[j] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int u = 0; u < D / 32; ++u) s[j] = Mat<T>::mma16(kf[i][j][u], qf[i][u], s[j]);
+      }
+      if (part || k0 + kTurn > end) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = k0 + 16 * j + 4 * g + e;
+            bool seen = key < limit && key < end;
+            if (mask) seen = seen && mask[(int64_t)min(key, a.k_len - 1) * a.ms[3]];
+            s[j][e] = seen ? s[j][e] : -INFINITY;
+          }
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, s[j][e]);
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      if (__any(top > m[i])) {
+        const float now = fmaxf(m[i], top), w = now == -INFINITY ? 1.0f : exp2_((m[i] - now) * a.c);
+        l[i] *= w;
+#pragma unroll
+        for (int t = 0; t < L::VT; ++t) acc[i][t] *= w;
+        m[i] = now;
+      }
+      const float mc = m[i] == -INFINITY ? 0.0f : m[i] * a.c;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = exp2_(fmaf(s[j][e], a.c, -mc));
+          l[i] += p;
+          pf[i][4 * j + e] = (T)p;
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                     // V has landed (this wave's own copies: no barrier)
+    if (part) {                                                          // infinities and NaN that a row does not see (see quarantine above)
+      auto finite16 = [](unsigned short u) { return std::is_same<T, bf16>::value ? (u & 0x7f80) != 0x7f80 : (u & 0x7c00) != 0x7c00; };
+      bool bad = false;
+      for (int p = lane; p < L::V_BYTES / 2; p += 64) bad |= !finite16(reinterpret_cast<const unsigned short*>(vt)[p]);
+      if (__any(bad)) {
+        for (int key = 0; key < kTurn; ++key) {
+          const bool seen = k0 + key < limit && k0 + key < end && (!mask || mask[(int64_t)(k0 + key) * a.ms[3]]);
+#pragma unroll
+          for (int t = 0; t < L::VT; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int dv = 16 * t + 4 * g + e;
+              const T val = reinterpret_cast<const T*>(vt + key * L::VP * 16)[8 * ((dv / 8) ^ L::v_swizzle(key)) + dv % 8];
+              if (seen && !finite16(__builtin_bit_cast(unsigned short, val))) { acc[0][t][e] += (float)val; acc[1][t][e] += (float)val; }
+            }
+        }
+        THA4_WAVE_SYNC();
+        for (int p = lane; p < L::V_BYTES / 2; p += 64) {
+          unsigned short* u = reinterpret_cast<unsigned short*>(vt) + p;
+          if (!finite16(*u)) *u = 0;
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < L::VT; ++t) {
+      const int r0 = 4 * g + ((lane & 15) >> 2), piece = 2 * t + ((lane & 3) >> 1), in = 8 * (lane & 1);
+      const s16x4 lo = read_transposed(vt + (r0 * L::VP + (piece ^ L::v_swizzle(r0))) * 16 + in);
+      const s16x4 hi = read_transposed(vt + ((r0 + 16) * L::VP + (piece ^ L::v_swizzle(r0 + 16))) * 16 + in);
+      const v8 vf = join<v8>(lo, hi);
+      acc[0][t] = Mat<T>::mma16(vf, pf[0], acc[0][t]);
+      acc[1][t] = Mat<T>::mma16(vf, pf[1], acc[1][t]);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                   // the next turn's copies overwrite what was read here
+  }
+
+  // the four waves meet: common maxima, then two rounds of sums
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l[i] += __shfl_xor(l[i], 16, 64);
+    l[i] += __shfl_xor(l[i], 32, 64);
+    if (lane < kRows) { stat[wave][2 * i][lane] = m[i]; stat[wave][2 * i + 1][lane] = l[i]; }
+  }
+  __syncthreads();
+  float M[2], S[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = lane & 15;
+    M[i] = fmaxf(fmaxf(stat[0][2 * i][r], stat[1][2 * i][r]), fmaxf(stat[2][2 * i][r], stat[3][2 * i][r]));
+    S[i] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) S[i] += stat[w][2 * i][r] == -INFINITY ? stat[w][2 * i + 1][r] : stat[w][2 * i + 1][r] * exp2_((stat[w][2 * i][r] - M[i]) * a.c);
+    const float w = m[i] == -INFINITY ? 1.0f : exp2_((m[i] - M[i]) * a.c);
+#pragma unroll
+    for (int t = 0; t < L::VT; ++t) acc[i][t] *= w;
+  }
+  f32x4* meet = reinterpret_cast<f32x4*>(lds) + (wave & 1) * (L::SET / 4) + lane;
+#pragma unroll
+  for (int round = 0; round < 2; ++round) {
+    const int givers = round == 0 ? 2 : 1;                               // waves 2, 3 give to 0, 1; then 1 gives to 0
+    if (wave >= givers && wave < 2 * givers) {
+      f32x4* to = reinterpret_cast<f32x4*>(lds) + (wave - givers) * (L::SET / 4) + lane;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int t = 0; t < L::VT; ++t) to[(i * L::VT + t) * 64] = acc[i][t];
+    }
+    __syncthreads();
+    if (wave < givers) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int t = 0; t < L::VT; ++t) acc[i][t] += meet[(i * L::VT + t) * 64];
+    }
+    __syncthreads();
+  }
+  if (wave) return;
+  if (a.splits == 1) {
+    finish_few<T, D>(a, acc, S[0], S[1], b, kv, R, rows, n.q);
+    return;
+  }
+  float* part = a.work + ((((int64_t)b * a.kv_heads + kv) * a.row_tiles + rt) * a.splits + split) * L::PART;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int t = 0; t < L::VT; ++t) reinterpret_cast<f32x4*>(part)[(i * L::VT + t) * 64 + lane] = acc[i][t];
+    if (lane < kRows) { part[L::SET + 2 * i * kRows + lane] = M[i]; part[L::SET + (2 * i + 1) * kRows + lane] = S[i]; }
+  }
+}
+
+// joins the ranges of the keys: the same rescaled sum over the ranges that hold keys, in their order
+template <class T, int D>
+__global__ void __launch_bounds__(64) diff_join_kernel(AttnArgs a) {
+  warm_kernarg<(int)sizeof(AttnArgs)>();
+  typedef Few<D> L;
+  const int lane = threadIdx.x;
+  int id = blockIdx.x;
+  const int rt = id % a.row_tiles; id /= a.row_tiles;
+  const int kv = id % a.kv_heads, b = id / a.kv_heads;
+  const Lengths n = lengths_of(a, b);
+  const int used = (n.k + a.chunk - 1) / a.chunk;
+  const float* part = a.work + (((int64_t)b * a.kv_heads + kv) * a.row_tiles + rt) * a.splits * L::PART;
+  f32x4 acc[2][L::VT];
+  float M[2] = {-INFINITY, -INFINITY}, S[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int t = 0; t < L::VT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
+    for (int s = 0; s < used; ++s) M[i] = fmaxf(M[i], part[s * L::PART + L::SET + 2 * i * kRows + (lane & 15)]);
+    for (int s = 0; s < used; ++s) {
+      const float* p = part + (int64_t)s * L::PART;
+      const float m = p[L::SET + 2 * i * kRows + (lane & 15)], l = p[L::SET + (2 * i + 1) * kRows + (lane & 15)];
+      const float w = m == -INFINITY ? 1.0f : exp2_((m - M[i]) * a.c);
+      S[i] += l * w;
+#pragma unroll
+      for (int t = 0; t < L::VT; ++t) acc[i][t] += w * reinterpret_cast<const f32x4*>(p)[(i * L::VT + t) * 64 + lane];
+    }
+  }
+  finish_few<T, D>(a, acc, S[0], S[1], b, kv, rt * kRows + lane % 16, a.q_len * a.group, n.q);
+}
+
+}  // namespace xf
+}  // namespace tha4

@@ -1,0 +1,212 @@
+"""Transformer block operators, without a GPU: what the entry points refuse, and the 64-bit oracle against direct statements of the definitions."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+import tha4_amd  # noqa: F401
+from oracle import transformer_oracle as oracle
+from tha4_amd import _capi, transformer
+
+
+@pytest.fixture(scope="module")
+def lib(built):
+    return _capi.load_library()
+
+
+def host(n=64):
+    """Host memory that no entry point may take for device memory."""
+    b = (C.c_char * n)()
+    return C.cast(b, C.c_void_p), b
+
+
+def refused(lib, status, *words):
+    assert status == -1
+    text = lib.tha4_last_error().decode()
+    for w in words:
+        assert w in text, text
+
+
+def test_quantize_refuses(lib):
+    p, keep = host()
+    q = lib.tha4_quantize_tokens_i8
+    refused(lib, q(p, 3, 1, 8, 8, p, 8, p, None), "x_dtype")
+    refused(lib, q(p, 0, -1, 8, 8, p, 8, p, None), "rows")
+    refused(lib, q(p, 0, 1, 0, 8, p, 8, p, None), "cols")
+    refused(lib, q(None, 0, 1, 8, 8, p, 8, p, None), "NULL")
+    refused(lib, q(p, 0, 1, 8, 8, p, 4, p, None), "q_row_stride")
+    refused(lib, q(p, 0, 1, 8, 8, p, 8, p, None), "device pointers")
+    assert q(None, 0, 0, 8, 8, None, 8, None, None) == 0                     # no rows: nothing to do
+
+
+def linear_args(p, **more):
+    a = dict(x_dev=p, x_scale_dev=p, w_dev=p, w_scale_dev=p, bias_dev=None, y_dev=p, m=1, n=1, k=1, x_row_stride=1, w_row_stride=1, y_row_stride=1, y_dtype=0)
+    a.update(more)
+    return C.byref(_capi.Tha4LinearI8Args(**{n: v.value if isinstance(v, C.c_void_p) else v for n, v in a.items()}))
+
+
+def test_linear_refuses(lib):
+    p, keep = host()
+    f = lib.tha4_linear_i8
+    refused(lib, f(None, None), "NULL")
+    refused(lib, f(linear_args(p, y_dtype=7), None), "y_dtype")
+    refused(lib, f(linear_args(p, k=0), None), "k must be positive")
+    refused(lib, f(linear_args(p, m=-1), None), "negative")
+    refused(lib, f(linear_args(p, k=131072), None), "131071")
+    refused(lib, f(linear_args(p, w_scale_dev=None), None), "NULL")
+    refused(lib, f(linear_args(p, n=2), None), "y_row_stride")
+    refused(lib, f(linear_args(p), None), "device pointers")
+    assert f(linear_args(None, m=0), None) == 0
+
+
+def norm_args(p, **more):
+    a = dict(residual_dev=p, branch_dev=p, h_dev=p, y_dev=p, rows=1, cols=8, residual_row_stride=8, branch_row_stride=8, h_row_stride=8, y_row_stride=8, gate_rows=1, film_rows=1,
+             residual_scale=1.0, eps=1e-5)
+    a.update(more)
+    return C.byref(_capi.Tha4ResidualNormArgs(**{n: v.value if isinstance(v, C.c_void_p) else v for n, v in a.items()}))
+
+
+def test_norm_refuses(lib):
+    p, keep = host()
+    f = lib.tha4_residual_norm
+    refused(lib, f(None, None), "NULL")
+    refused(lib, f(norm_args(p, dtype=9), None), "dtype")
+    refused(lib, f(norm_args(p, residual_dtype=1), None), "residual_dtype")
+    refused(lib, f(norm_args(p, post_norm=3), None), "norm")
+    refused(lib, f(norm_args(p, gate_activation=2), None), "gate")
+    refused(lib, f(norm_args(p, cols=0), None), "cols")
+    refused(lib, f(norm_args(p, eps=-1.0), None), "eps")
+    refused(lib, f(norm_args(p, eps=math.nan), None), "eps")
+    refused(lib, f(norm_args(p, residual_scale=math.inf), None), "residual_scale")
+    refused(lib, f(norm_args(p, residual_dev=None), None), "residual")
+    refused(lib, f(norm_args(p, branch_dev=None, gate_dev=p), None), "branch")
+    refused(lib, f(norm_args(p, film_scale_dev=p), None), "together")
+    refused(lib, f(norm_args(p, y_dev=None, pre_weight_dev=p), None), "need y")
+    refused(lib, f(norm_args(p, h_dev=None, y_dev=None), None), "one of h and y")
+    refused(lib, f(norm_args(p, gate_dev=p, gate_rows=0), None), "gate_rows")
+    refused(lib, f(norm_args(p, y_row_stride=4), None), "strides")
+    refused(lib, f(norm_args(p, residual_row_stride=-8), None), "negative")
+    refused(lib, f(norm_args(p), None), "device pointers")
+    assert f(norm_args(None, rows=0), None) == 0
+
+
+def attention_args(p, **more):
+    a = dict(q_dev=p, k_dev=p, v_dev=p, out_dev=p, lambda_vectors_dev=p, dtype=2, batch=1, q_len=1, k_len=1, heads=1, kv_heads=1, head_dim=32, scale=1.0, lambda_init=0.5, eps=1e-5)
+    a.update(more)
+    return C.byref(_capi.Tha4DiffAttentionArgs(**{n: v.value if isinstance(v, C.c_void_p) else v for n, v in a.items()}))
+
+
+def test_attention_refuses(lib):
+    p, keep = host(256)
+    p = C.c_void_p((p.value + 15) // 16 * 16)
+    f = lib.tha4_diff_attention
+    refused(lib, f(None, None), "NULL")
+    assert lib.tha4_diff_attention_workspace(None) == -1
+    for call in (lambda a: f(a, None), lib.tha4_diff_attention_workspace):
+        refused(lib, call(attention_args(p, dtype=0)), "f16 or bf16")
+        refused(lib, call(attention_args(p, head_dim=48)), "head_dim")
+        refused(lib, call(attention_args(p, heads=3, kv_heads=2)), "multiple")
+        refused(lib, call(attention_args(p, kv_heads=0)), "kv_heads")
+        refused(lib, call(attention_args(p, q_len=-1)), "negative")
+    refused(lib, f(attention_args(p, scale=0.0), None), "scale")
+    refused(lib, f(attention_args(p, scale=math.nan), None), "scale")
+    refused(lib, f(attention_args(p, eps=-1.0), None), "eps")
+    refused(lib, f(attention_args(p, lambda_init=math.inf), None), "lambda_init")
+    refused(lib, f(attention_args(p, q_dev=None), None), "NULL")
+    refused(lib, f(attention_args(p, k_dev=None), None), "k / v")
+    refused(lib, f(attention_args(C.c_void_p(p.value + 2)), None), "aligned")
+    refused(lib, f(attention_args(p, k_stride=(C.c_int64 * 3)(8, 4, 8)), None), "multiples of 8")
+    refused(lib, f(attention_args(p, k_stride=(C.c_int64 * 3)(8, 1 << 24, 8)), None), "2^24")
+    refused(lib, f(attention_args(p, k_stride=(C.c_int64 * 3)(-8, 8, 8)), None), "negative")
+    refused(lib, f(attention_args(p, k_len=1 << 20), None), "workspace")     # few queries over a long cache: its ranges meet in a workspace
+    refused(lib, f(attention_args(p), None), "device pointers")
+    assert f(attention_args(p, batch=0), None) == 0
+    assert f(attention_args(p, q_len=0), None) == 0
+
+
+def test_workspace_is_a_function_of_the_sizes(lib):
+    a = attention_args(None, k_len=131072, batch=2, heads=8, kv_heads=2, head_dim=128)
+    n = lib.tha4_diff_attention_workspace(a)
+    assert n > 0 and n == lib.tha4_diff_attention_workspace(a)
+    assert lib.tha4_diff_attention_workspace(attention_args(None, q_len=512, k_len=512)) == 0
+
+
+def test_python_refuses_cpu_tensors_and_wrong_shapes(lib):
+    x = torch.zeros(2, 32)
+    w, ws = torch.zeros(4, 32, dtype=torch.int8), torch.ones(4)
+    with pytest.raises(AssertionError, match="GPU"):
+        transformer.quantize_tokens(x)
+    with pytest.raises(AssertionError, match="float32, float16 or bfloat16"):
+        transformer.quantize_tokens(x.double())
+    with pytest.raises(AssertionError, match="GPU"):
+        transformer.int8_linear(x, w, ws)
+    with pytest.raises(AssertionError, match=r"\[\.\.\., 32\]"):
+        transformer.int8_linear(torch.zeros(2, 31), w, ws)
+    with pytest.raises(AssertionError, match="weight_scale"):
+        transformer.int8_linear(x, w, torch.ones(5))
+    with pytest.raises(AssertionError, match="GPU"):
+        transformer.residual_norm(x)
+    with pytest.raises(AssertionError, match="shape"):
+        transformer.residual_norm(x, torch.zeros(3, 32))
+    with pytest.raises(AssertionError, match="post_norm"):
+        transformer.residual_norm(x, x, post_norm="batch")
+    with pytest.raises(AssertionError, match="all be float32"):
+        transformer.residual_norm(x, x, pre_weight=torch.ones(32), post_weight=torch.ones(32, dtype=torch.bfloat16))
+    q = torch.zeros(1, 3, 4, 32, dtype=torch.bfloat16)
+    v = torch.zeros(1, 3, 2, 64, dtype=torch.bfloat16)
+    lam = torch.zeros(4, 32)
+    with pytest.raises(AssertionError, match="GPU"):
+        transformer.differential_attention(q, q, v, lam, 0.5)
+    with pytest.raises(AssertionError, match="float16"):
+        transformer.differential_attention(q.float(), q.float(), v.float(), lam, 0.5)
+    with pytest.raises(AssertionError, match="v \\[batch"):
+        transformer.differential_attention(q, q, v[..., :32], lam, 0.5)
+    with pytest.raises(AssertionError, match="pairs"):
+        transformer.differential_attention(q[:, :, :3], q, v, lam, 0.5)
+    with pytest.raises(AssertionError, match="lambda_vectors"):
+        transformer.differential_attention(q, q, v, lam[:2], 0.5)
+    with pytest.raises(AssertionError, match="int32"):
+        transformer.differential_attention(q, q, v, lam, 0.5, kv_lengths=torch.ones(1))
+
+
+def test_oracle_quantize_rounds_the_exact_quotient():
+    from fractions import Fraction
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(6, 40, generator=g)
+    x[1] = x[1].to(torch.bfloat16).float()
+    x[2, 3], x[2, 4] = x[2].abs().max(), x[2].abs().max() / 2            # half of the largest: next to a tie
+    x[3] *= 2.0 ** -140                                                    # a scale among the subnormals
+    x[4] = 0
+    q, s = oracle.quantize(x)
+    for r in range(6):
+        for c in range(40):
+            if float(s[r]) == 0:
+                assert q[r, c] == 0
+                continue
+            t = Fraction(float(x[r, c])) / Fraction(float(s[r]))
+            assert int(q[r, c]) == max(-127, min(127, round(t)))           # Fraction rounds ties to even
+
+
+def test_oracle_attention_against_a_direct_statement():
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(2, 5, n, d, generator=g).double() for n, d in ((4, 32), (2, 32), (1, 64)))
+    k, v = torch.cat([k, k], 1)[:, :7], torch.cat([v, v], 1)[:, :7]
+    lam, w = torch.randn(4, 2, 32, generator=g) * 0.1, torch.rand(64, generator=g)
+    mask = torch.rand(2, 1, 5, 7, generator=g) > 0.3
+    q, k, v = q.half(), k.half(), v.half()
+    out, bound = oracle.differential_attention(q, k, v, lam, 0.4, causal=True, kv_lengths=torch.tensor([7, 3]), mask=mask, norm_weight=w)
+    for b in range(2):
+        n = (7, 3)[b]
+        for h in range(2):
+            la = math.exp(float(lam[0, h].double() @ lam[1, h].double())) - math.exp(float(lam[2, h].double() @ lam[3, h].double())) + 0.4
+            for i in range(5):
+                see = [j for j in range(n) if j <= i + n - 5 and mask[b, 0, i, j]]
+                o = torch.zeros(64, dtype=torch.float64)
+                for m, sign in ((0, 1.0), (1, -la)):
+                    if see:
+                        p = torch.softmax((k[b, see, m].double() @ q[b, i, 2 * h + m].double()) / math.sqrt(32), 0)
+                        o += sign * (p @ v[b, see, 0].double())
+                o = 0.6 * o / torch.sqrt((o * o).mean() + 1e-5) * w
+                assert torch.allclose(out[b, i, h], o, atol=1e-12)
+    assert (bound >= 0).all() and float(bound.max()) < 0.02
