@@ -313,18 +313,24 @@ int tha4_quantize_tokens_i8(const void* x_dev, int x_dtype, int64_t rows, int64_
                             float* scale_dev, void* stream);
 
 /* y[i][j] = x_scale[i] w_scale[j] sum_k x[i][k] w[j][k] + bias[j]: int8 x int8 with exact int32 sums (k <= 131071), scaled in fp32 and rounded once
- * to y_dtype.  Any strides and alignments are valid; rows that are 16-byte aligned take the fast path. */
+ * to y_dtype.  x is int8 (x_dtype THA4_I8) with x_scale, or float (x_scale NULL): then it is quantised for each token on the way, as tha4_quantize_tokens_i8 would,
+ * for which more than a few tokens need tha4_linear_i8_workspace() bytes, 16-byte aligned.  Any strides (elements) and alignments are valid; k a multiple
+ * of 16 and 16-byte aligned rows take the fast path. */
+#define THA4_I8 3
 typedef struct tha4_linear_i8_args {
-  const int8_t* x_dev;          /* [m][k] */
+  const void* x_dev;            /* [m][k] */
   const float* x_scale_dev;     /* [m]    */
   const int8_t* w_dev;          /* [n][k] */
   const float* w_scale_dev;     /* [n]    */
   const float* bias_dev;        /* [n] or NULL */
   void* y_dev;                  /* [m][n] */
+  void* workspace_dev;
+  int64_t workspace_bytes;
   int64_t m, n, k;
   int64_t x_row_stride, w_row_stride, y_row_stride;
-  int32_t y_dtype;
+  int32_t x_dtype, y_dtype;
 } tha4_linear_i8_args;
+int64_t tha4_linear_i8_workspace(const tha4_linear_i8_args* args);
 int tha4_linear_i8(const tha4_linear_i8_args* args, void* stream);
 
 /* The norms behind and in front of a block, with the gate and the residual sum between them:

@@ -52,14 +52,15 @@ class Tha4StudentAux(C.Structure):
 ERR_NUMERIC_RANGE = -5
 
 # ---- operators of a transformer block (tha4_amd.transformer) ----
-F32, F16, BF16 = 0, 1, 2
+F32, F16, BF16, I8 = 0, 1, 2, 3
 NORM_KINDS = {"none": 0, "rms": 1, "layer": 2}
 GATE_ACTIVATIONS = {"none": 0, "sigmoid": 1}
 
 
 class Tha4LinearI8Args(C.Structure):
-    _fields_ = [(n, C.c_void_p) for n in ("x_dev", "x_scale_dev", "w_dev", "w_scale_dev", "bias_dev", "y_dev")] + \
-               [(n, C.c_int64) for n in ("m", "n", "k", "x_row_stride", "w_row_stride", "y_row_stride")] + [("y_dtype", C.c_int32)]
+    _fields_ = [(n, C.c_void_p) for n in ("x_dev", "x_scale_dev", "w_dev", "w_scale_dev", "bias_dev", "y_dev", "workspace_dev")] + \
+               [(n, C.c_int64) for n in ("workspace_bytes", "m", "n", "k", "x_row_stride", "w_row_stride", "y_row_stride")] + \
+               [("x_dtype", C.c_int32), ("y_dtype", C.c_int32)]
 
 
 class Tha4ResidualNormArgs(C.Structure):
@@ -260,6 +261,8 @@ def load_library(path: Optional[str] = None) -> C.CDLL:
     lib.tha4_ingest_rgba8.argtypes = [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]
     lib.tha4_quantize_tokens_i8.restype = C.c_int
     lib.tha4_quantize_tokens_i8.argtypes = [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]
+    lib.tha4_linear_i8_workspace.restype = C.c_int64
+    lib.tha4_linear_i8_workspace.argtypes = [C.POINTER(Tha4LinearI8Args)]
     lib.tha4_linear_i8.restype = C.c_int
     lib.tha4_linear_i8.argtypes = [C.POINTER(Tha4LinearI8Args), C.c_void_p]
     lib.tha4_residual_norm.restype = C.c_int
@@ -282,7 +285,7 @@ EXPORTED_SYMBOLS = [
     "tha4_full_create", "tha4_full_create_ex", "tha4_full_num_networks", "tha4_full_flags", "tha4_full_set_fault_policy", "tha4_full_set_timing", "tha4_full_num_ops", "tha4_full_op_info", "tha4_full_last_op_ms", "tha4_full_pose", "tha4_full_pose_ex", "tha4_full_numeric_status",
     "tha4_full_destroy", "tha4_full_max_batch",
     "tha4_display_rgba8", "tha4_ingest_rgba8",
-    "tha4_quantize_tokens_i8", "tha4_linear_i8", "tha4_residual_norm", "tha4_diff_attention_workspace", "tha4_diff_attention",
+    "tha4_quantize_tokens_i8", "tha4_linear_i8_workspace", "tha4_linear_i8", "tha4_residual_norm", "tha4_diff_attention_workspace", "tha4_diff_attention",
 ]
 
 

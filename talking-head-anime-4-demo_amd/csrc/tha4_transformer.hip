@@ -4,6 +4,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <string>
 
@@ -59,6 +60,38 @@ int quantize(const QuantArgs& a, void* stream) {
   return launch(quantize_kernel<T, 1024, 2>, a.rows, 1, 1024, a, stream);
 }
 
+// ---- product ----
+const char* check_linear(const tha4_linear_i8_args& g) {
+  if (g.x_dtype != THA4_I8 && !known(g.x_dtype)) return "x_dtype must be i8, f32, f16 or bf16";
+  if (!known(g.y_dtype)) return "y_dtype must be f32, f16 or bf16";
+  if (g.m < 0 || g.n < 0 || g.k < 1) return "m / n must not be negative and k must be positive";
+  if (g.k > 131071) return "k must be at most 131071 (the sums are 32-bit integers)";
+  if (g.m > kMaxGrid || g.n > kMaxGrid) return "m / n must be below 2^31";
+  return nullptr;
+}
+// float tokens that every workgroup of the product quantises for itself (linear_few_kernel)
+bool inline_tokens(const tha4_linear_i8_args& g) { return g.m <= kInlineTokens && g.m * g.k <= kInlineBytes; }
+int64_t token_stride(const tha4_linear_i8_args& g) { return ceil_div(g.k, 16) * 16; }
+
+template <class XT, int MT, bool INLINE>
+int few(const LinearArgs& a, bool al, void* stream) {
+  const int64_t nb = ceil_div(a.n, 16), mb = ceil_div(a.m, 16 * MT);
+  return al ? launch(linear_few_kernel<XT, MT, true, INLINE>, nb, mb, 512, a, stream) : launch(linear_few_kernel<XT, MT, false, INLINE>, nb, mb, 512, a, stream);
+}
+template <int BM, int BN, int WM, int WN, int STAGES>
+int tile(const LinearArgs& a, bool al, void* stream) {
+  const int64_t tiles = ceil_div(a.m, BM) * ceil_div(a.n, BN);
+  return al ? launch(linear_tile_kernel<BM, BN, WM, WN, STAGES, true>, tiles, 1, 64 * WM * WN, a, stream)
+            : launch(linear_tile_kernel<BM, BN, WM, WN, STAGES, false>, tiles, 1, 64 * WM * WN, a, stream);
+}
+int product(const LinearArgs& a, bool al, void* stream) {
+  if (a.m <= 16) return few<float, 1, false>(a, al, stream);
+  if (a.m <= 64) return few<float, 4, false>(a, al, stream);
+  if (al && ceil_div(a.m, 256) * ceil_div(a.n, 256) >= 192) return tile<256, 256, 2, 4, 4>(a, al, stream);
+  if (ceil_div(a.m, 128) * ceil_div(a.n, 128) >= 192) return tile<128, 128, 2, 2, 4>(a, al, stream);
+  return tile<64, 64, 2, 2, 4>(a, al, stream);
+}
+
 // ---- norms ----
 template <class T, class R>
 int norm(const NormArgs& a, bool vector, void* stream) {
@@ -74,7 +107,7 @@ int norm(const NormArgs& a, bool vector, void* stream) {
 // How the keys are divided among workgroups when there are few queries.  A pure function of the sizes: the workspace query and the launch agree.
 struct Plan {
   bool few;
-  int row_tiles, splits, chunk;
+  int row_tiles, splits, chunk, part_rows;
 };
 Plan plan_of(const tha4_diff_attention_args& a) {
   Plan p{};
@@ -84,12 +117,11 @@ Plan plan_of(const tha4_diff_attention_args& a) {
   p.chunk = a.k_len;
   if (!p.few) return p;
   p.row_tiles = (int)ceil_div(rows, kRows);
-  const int64_t wgs = (int64_t)a.batch * a.kv_heads * p.row_tiles;
-  const int64_t want = ceil_div(1024, wgs);
-  int64_t chunk = ceil_div(ceil_div(a.k_len, want), 128) * 128;
-  if (chunk < 512) chunk = 512;
-  p.splits = (int)ceil_div(a.k_len, chunk);
-  if (p.splits < 1) p.splits = 1;
+  p.part_rows = (int)std::min<int64_t>(rows, kRows);
+  const int64_t wgs = std::max<int64_t>((int64_t)a.batch * a.kv_heads * p.row_tiles, 1);
+  const int64_t want = std::min<int64_t>(ceil_div(a.kv_lengths_dev ? 2048 : 1024, wgs), kMaxSplits);
+  const int64_t chunk = std::max<int64_t>(ceil_div(ceil_div(a.k_len, want), 128) * 128, 256);
+  p.splits = (int)std::max<int64_t>(ceil_div(a.k_len, chunk), 1);
   p.chunk = (int)chunk;
   return p;
 }
@@ -111,7 +143,7 @@ int attention(AttnArgs& a, const Plan& p, void* stream) {
   const int64_t tiles = (int64_t)a.batch * a.kv_heads * p.row_tiles;
   const int st = launch(diff_few_kernel<T, D>, tiles * p.splits, 1, 256, a, stream);
   if (st != THA4_OK || p.splits == 1) return st;
-  return launch(diff_join_kernel<T, D>, tiles, 1, 64, a, stream);
+  return launch(diff_join_kernel<T, D>, tiles * p.part_rows, 1, 512, a, stream);
 }
 template <class T>
 int attention(AttnArgs& a, int d, const Plan& p, void* stream) {
@@ -136,27 +168,43 @@ int tha4_quantize_tokens_i8(const void* x_dev, int x_dtype, int64_t rows, int64_
   return x_dtype == THA4_F32 ? quantize<float>(a, stream) : x_dtype == THA4_F16 ? quantize<f16>(a, stream) : quantize<bf16>(a, stream);
 }
 
+int64_t tha4_linear_i8_workspace(const tha4_linear_i8_args* args) {
+  if (!args) return bad("args must not be NULL");
+  if (const char* e = check_linear(*args)) return bad(e);
+  return args->x_dtype == THA4_I8 || inline_tokens(*args) ? 0 : args->m * (token_stride(*args) + 4);
+}
+
 int tha4_linear_i8(const tha4_linear_i8_args* args, void* stream) {
   if (!args) return bad("args must not be NULL");
   const tha4_linear_i8_args& g = *args;
-  if (!known(g.y_dtype)) return bad("y_dtype must be f32, f16 or bf16");
-  if (g.m < 0 || g.n < 0 || g.k < 1) return bad("m / n must not be negative and k must be positive");
-  if (g.k > 131071) return bad("k must be at most 131071 (the sums are 32-bit integers)");
+  if (const char* e = check_linear(g)) return bad(e);
   if (g.m == 0 || g.n == 0) return THA4_OK;
-  if (!g.x_dev || !g.x_scale_dev || !g.w_dev || !g.w_scale_dev || !g.y_dev) return bad("x / x_scale / w / w_scale / y must not be NULL");
+  const bool quantised = g.x_dtype == THA4_I8;
+  if (!g.x_dev || !g.w_dev || !g.w_scale_dev || !g.y_dev) return bad("x / w / w_scale / y must not be NULL");
+  if (quantised != (g.x_scale_dev != nullptr)) return bad("x_scale belongs to an int8 x, and only there");
   if (g.x_row_stride < 0 || g.w_row_stride < 0 || g.y_row_stride < g.n) return bad("row strides must not be negative and y_row_stride must be at least n");
-  const int dev = one_device({g.x_dev, g.x_scale_dev, g.w_dev, g.w_scale_dev, g.bias_dev, g.y_dev});
-  if (dev < 0) return bad("x / x_scale / w / w_scale / bias / y must be device pointers of one GPU");
+  const int64_t need = tha4_linear_i8_workspace(args);
+  if (need && (!g.workspace_dev || g.workspace_bytes < need || reinterpret_cast<uintptr_t>(g.workspace_dev) % 16))
+    return bad("workspace is smaller than tha4_linear_i8_workspace() or not 16-byte aligned");
+  const int dev = one_device({g.x_dev, g.x_scale_dev, g.w_dev, g.w_scale_dev, g.bias_dev, g.y_dev, need ? g.workspace_dev : nullptr});
+  if (dev < 0) return bad("x / x_scale / w / w_scale / bias / y / workspace must be device pointers of one GPU");
   DeviceGuard guard(dev);
-  const LinearArgs a{g.x_dev, g.w_dev, g.x_scale_dev, g.w_scale_dev, g.bias_dev, g.y_dev, g.m, g.n, g.k, g.x_row_stride, g.w_row_stride, g.y_row_stride, g.y_dtype};
-  const bool al = g.k % 16 == 0 && aligned(g.x_dev, g.x_row_stride, 1) && aligned(g.w_dev, g.w_row_stride, 1);
-  if (g.m <= 64) {
-    const int64_t nb = ceil_div(g.n, 16);
-    if (g.m <= 16) return al ? launch(linear_few_kernel<1, true>, nb, 1, 512, a, stream) : launch(linear_few_kernel<1, false>, nb, 1, 512, a, stream);
-    return al ? launch(linear_few_kernel<4, true>, nb, 1, 512, a, stream) : launch(linear_few_kernel<4, false>, nb, 1, 512, a, stream);
+  LinearArgs a{g.x_dev, g.w_dev, g.x_scale_dev, g.w_scale_dev, g.bias_dev, g.y_dev, g.m, g.n, g.k, g.x_row_stride, g.w_row_stride, g.y_row_stride, g.x_dtype, g.y_dtype};
+  const bool w16 = g.k % 16 == 0 && aligned(g.w_dev, g.w_row_stride, 1);
+  if (!quantised) {
+    if (inline_tokens(g))
+      return g.x_dtype == THA4_F32 ? few<float, 1, true>(a, w16, stream) : g.x_dtype == THA4_F16 ? few<f16, 1, true>(a, w16, stream) : few<bf16, 1, true>(a, w16, stream);
+    const int64_t stride = token_stride(g);
+    int8_t* q = static_cast<int8_t*>(g.workspace_dev);
+    float* scale = reinterpret_cast<float*>(q + g.m * stride);
+    const QuantArgs t{g.x_dev, q, scale, g.m, g.k, g.x_row_stride, stride};
+    const int st = g.x_dtype == THA4_F32 ? quantize<float>(t, stream) : g.x_dtype == THA4_F16 ? quantize<f16>(t, stream) : quantize<bf16>(t, stream);
+    if (st != THA4_OK) return st;
+    a.x = q;
+    a.xs = scale;
+    a.x_stride = stride;
   }
-  const int64_t nb = ceil_div(g.n, 128), mb = ceil_div(g.m, 128);
-  return al ? launch(linear_tile_kernel<true>, nb, mb, 256, a, stream) : launch(linear_tile_kernel<false>, nb, mb, 256, a, stream);
+  return product(a, w16 && aligned(a.x, a.x_stride, 1), stream);
 }
 
 int tha4_residual_norm(const tha4_residual_norm_args* args, void* stream) {
@@ -202,7 +250,7 @@ int64_t tha4_diff_attention_workspace(const tha4_diff_attention_args* args) {
   if (!args) return bad("args must not be NULL");
   if (const char* e = check_shape(*args)) return bad(e);
   const Plan p = plan_of(*args);
-  return p.splits == 1 ? 0 : (int64_t)args->batch * args->kv_heads * p.row_tiles * p.splits * part_floats(args->head_dim) * 4;
+  return p.splits == 1 ? 0 : (int64_t)args->batch * args->kv_heads * p.row_tiles * p.part_rows * p.splits * part_floats(args->head_dim) * 4;
 }
 
 int tha4_diff_attention(const tha4_diff_attention_args* args, void* stream) {
@@ -243,7 +291,7 @@ int tha4_diff_attention(const tha4_diff_attention_args* args, void* stream) {
   a.lambda_vs = g.lambda_vector_stride; a.lambda_hs = g.lambda_head_stride;
   a.batch = g.batch; a.q_len = g.q_len; a.k_len = g.k_len; a.heads = g.heads; a.kv_heads = g.kv_heads; a.group = g.heads / g.kv_heads;
   a.causal = g.causal; a.norm = g.norm;
-  a.row_tiles = p.row_tiles; a.splits = p.splits; a.chunk = p.chunk;
+  a.row_tiles = p.row_tiles; a.splits = p.splits; a.chunk = p.chunk; a.part_rows = p.part_rows;
   a.c = g.scale * 1.44269504088896340736f; a.lambda_init = g.lambda_init; a.eps = g.eps;
   return g.dtype == THA4_F16 ? attention<f16>(a, g.head_dim, p, stream) : attention<bf16>(a, g.head_dim, p, stream);
 }

@@ -23,7 +23,7 @@ struct AttnArgs {
   int64_t qs[3], ks[3], vs[3], os[3], ms[4];
   int64_t lambda_vs, lambda_hs;
   int32_t batch, q_len, k_len, heads, kv_heads, group, causal, norm;
-  int32_t row_tiles, splits, chunk;
+  int32_t row_tiles, splits, chunk, part_rows;
   float c, lambda_init, eps;                   // c = scale * log2(e): the softmax is taken in powers of two
 };
 
@@ -292,25 +292,42 @@ __global__ void __launch_bounds__(512, 2) diff_prompt_kernel(AttnArgs a) {
 
 // ---- few queries over a long cache -------------------------------------------------------------------------------------------------------
 // The cache is the traffic: 4 d elements a key and kv head, read once for all queries and heads that share it (up to 16 rows, the columns of the 16 x 16 x 32 products).
-// A workgroup owns a range of the keys; its four waves take turns of 32 keys, each with running statistics of its own and without barriers: K from memory into
-// operand registers, V through the wave's own LDS for the transposing read.  The waves meet in LDS, the ranges in a second launch.
-constexpr int kTurn = 32, kRows = 16;
+// A workgroup owns a range of the keys; its four waves take turns of 32 keys, each with running statistics and LDS of its own and without barriers.  The next turn's K is
+// requested as soon as this turn's has been read into operands, the next V behind the product with this one: a wave always has one of the two in flight,
+// asynchronously and straight into LDS, behind counted waits.  The waves meet in LDS, the ranges in a second launch.
+constexpr int kTurn = 32, kRows = 16, kMaxSplits = 512;
 
 template <int D>
 struct Few {
-  static constexpr int VP = D / 4, VT = D / 8;                         // pieces of a V row; tiles of 16 value columns
-  static constexpr int V_BYTES = kTurn * VP * 16;                      // one wave's V
-  static constexpr int SET = 2 * VT * 4 * 64;                          // floats of one wave's (or range's) two accumulators
-  static constexpr int PART = SET + 4 * kRows;                         // ... and their statistics: m1, l1, m2, l2 of each row
+  static constexpr int KP = D / 8, VP = D / 4, VT = D / 8;             // 16-byte pieces of a K row (one map), of a V row; tiles of 16 value columns
+  static constexpr int K_COPIES = KP, V_COPIES = VP / 2;               // KiB of a turn's K (both maps), V
+  static constexpr int WAVE_BYTES = (K_COPIES + V_COPIES) * 1024;
+  static constexpr int SET = 2 * VT * 4 * 64;                          // floats of one wave's two accumulators
+  static constexpr int PART = 4 * D + 4;                               // floats that a range leaves for each row: O1, O2, m1, l1, m2, l2
+  // slots of the 16 lanes that the LDS serves together (rows 0 - 3 and 12 - 15 of one piece, 4 - 11 of the next one) all differ
+  static THA4_DEV int k_swizzle(int row) { return KP == 4 ? (4 - (row >> 2)) & 3 : (row / (16 / KP)) & (KP - 1); }
   static THA4_DEV int v_swizzle(int row) { return VP == 8 ? ((row >> 1) & 3) * 2 : (row & 7) * 2; }
 };
+
+// A query's value columns: o = O1 w1 - O2 w2, normalised and stored, 4 columns a lane and step.  `ss` sums over the lanes that share the query.
+template <class T, int D>
+THA4_DEV void store_columns(const AttnArgs& a, T* out, int dv, const f32x4& o, float g) {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  T4 r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) r[e] = (T)(o[e] * g * (a.norm && a.norm_w ? a.norm_w[dv + e] : 1.0f));
+  *reinterpret_cast<T4*>(out + dv) = r;
+}
+template <int D>
+THA4_DEV float norm_factor(const AttnArgs& a, float ss) { return a.norm ? (1.0f - a.lambda_init) / sqrtf(ss * (1.0f / (2 * D)) + a.eps) : 1.0f; }
+THA4_DEV float weight_of(float top, float l) { return l > 0.0f || l != l ? top / l : 0.0f; }      // (no key seen: nothing)
 
 // out of O1, l1, O2, l2 (accumulator layout: row lane % 16, value columns 16 t + 4 (lane / 16) + e)
 template <class T, int D>
 THA4_DEV void finish_few(const AttnArgs& a, f32x4 (&o)[2][D / 8], float l1, float l2, int b, int kv, int R, int rows, int q_valid) {
   const int lane = threadIdx.x & 63, head = kv * a.group + R % a.group, qi = R / a.group;
-  // (every lane of the wave takes part in the sums of lambda: the heads of a wave's rows differ)
-  const float* l = a.lambdas + min(head, a.heads - 1) * a.lambda_hs;
+  // (every lane takes part in the sums of lambda: the heads of a wave's rows differ)
+  const float* l = a.lambdas + head * a.lambda_hs;
   float s = 0.0f, t2 = 0.0f;
   for (int i = lane >> 4; i < D; i += 4) {
     s = fmaf(l[i], l[a.lambda_vs + i], s);
@@ -318,8 +335,7 @@ THA4_DEV void finish_few(const AttnArgs& a, f32x4 (&o)[2][D / 8], float l1, floa
   }
   s += __shfl_xor(s, 16, 64); s += __shfl_xor(s, 32, 64);
   t2 += __shfl_xor(t2, 16, 64); t2 += __shfl_xor(t2, 32, 64);
-  const float lam = expf(s) - expf(t2) + a.lambda_init;
-  const float w1 = l1 > 0.0f || l1 != l1 ? 1.0f / l1 : 0.0f, w2 = l2 > 0.0f || l2 != l2 ? lam / l2 : 0.0f;
+  const float w1 = weight_of(1.0f, l1), w2 = weight_of(expf(s) - expf(t2) + a.lambda_init, l2);
   float ss = 0.0f;
 #pragma unroll
   for (int t = 0; t < D / 8; ++t)
@@ -331,31 +347,49 @@ THA4_DEV void finish_few(const AttnArgs& a, f32x4 (&o)[2][D / 8], float l1, floa
   ss += __shfl_xor(ss, 16, 64);
   ss += __shfl_xor(ss, 32, 64);
   if (R >= rows || qi >= q_valid) return;
-  const float g = a.norm ? (1.0f - a.lambda_init) / sqrtf(ss * (1.0f / (2 * D)) + a.eps) : 1.0f;
+  const float g = norm_factor<D>(a, ss);
   T* out = static_cast<T*>(a.out) + b * a.os[0] + qi * a.os[1] + head * a.os[2];
-  typedef T T4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-  for (int t = 0; t < D / 8; ++t) {
-    const int dv = 16 * t + 4 * (lane >> 4);
-    T4 r;
+  for (int t = 0; t < D / 8; ++t) store_columns<T, D>(a, out, 16 * t + 4 * (lane >> 4), o[0][t], g);
+}
+
+// One wave's K or V of a turn: `left` is the last valid row (rows behind it repeat it).  Offsets inside a turn fit 32 bits (the host bounds the strides).
+template <class T, int D>
+THA4_DEV void request_k(const AttnArgs& a, const T* k, int left, unsigned lds) {
+  typedef Few<D> L;
+  const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = (T)(o[0][t][e] * g * (a.norm && a.norm_w ? a.norm_w[dv + e] : 1.0f));
-    *reinterpret_cast<T4*>(out + dv) = r;
+  for (int u = 0; u < L::K_COPIES; ++u) {
+    const int p = u * 64 + lane, map = p / (kTurn * L::KP), row = (p / L::KP) % kTurn, pos = p % L::KP;
+    copy16_async(k + map * a.ks[2] + ((unsigned)min(row, left) * (unsigned)a.ks[1] + 8 * (pos ^ L::k_swizzle(row % 16))), lds + u * 1024);
   }
 }
+template <class T, int D>
+THA4_DEV void request_v(const AttnArgs& a, const T* v, int left, unsigned lds) {
+  typedef Few<D> L;
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int u = 0; u < L::V_COPIES; ++u) {
+    const int p = u * 64 + lane, row = p / L::VP, pos = p % L::VP;
+    copy16_async(v + ((unsigned)min(row, left) * (unsigned)a.vs[1] + 8 * (pos ^ L::v_swizzle(row))), lds + u * 1024);
+  }
+}
+template <int N>
+THA4_DEV void wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }       // at most the N newest requests of this wave are on their way
+THA4_DEV void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }               // what this wave read from LDS has arrived: it may be overwritten
 
 template <class T, int D>
 __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArgs a) {
   warm_kernarg<(int)sizeof(AttnArgs)>();
   typedef Few<D> L;
   typedef typename Mat<T>::v8 v8;
-  constexpr int LDS = 4 * L::V_BYTES > 2 * L::SET * 4 ? 4 * L::V_BYTES : 2 * L::SET * 4;
+  constexpr int LDS = 4 * L::WAVE_BYTES > 2 * L::SET * 4 ? 4 * L::WAVE_BYTES : 2 * L::SET * 4;
   __shared__ __attribute__((aligned(16))) char lds[LDS];
   __shared__ float stat[4][4][kRows];
   const int lane = threadIdx.x & 63, wave = uniform_i32(threadIdx.x >> 6), g = lane >> 4;
   int id = blockIdx.x;
   const int split = id % a.splits; id /= a.splits;
-  const int rt = id % a.row_tiles; id /= a.row_tiles;
+  const int rt = id % a.row_tiles, tile = id; id /= a.row_tiles;
   const int kv = id % a.kv_heads, b = id / a.kv_heads;
   const Lengths n = lengths_of(a, b);
   const int rows = a.q_len * a.group, R = rt * kRows + (lane & 15), Rc = min(R, rows - 1);
@@ -369,6 +403,14 @@ __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArg
   const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + 2 * kv * a.ks[2];
   const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2];
   const uint8_t* mask = a.mask ? a.mask + b * a.ms[0] + head * a.ms[1] + qi * a.ms[2] : nullptr;
+  char* kt = lds + wave * L::WAVE_BYTES;
+  char* vt = kt + L::K_COPIES * 1024;
+  const unsigned kt_at = lds_address(kt), vt_at = lds_address(vt);
+  int k0 = begin + wave * kTurn;
+  if (k0 < end) {
+    request_k<T, D>(a, k + (int64_t)k0 * a.ks[1], n.k - 1 - k0, kt_at);
+    request_v<T, D>(a, v + (int64_t)k0 * a.vs[1], n.k - 1 - k0, vt_at);
+  }
   v8 qf[2][D / 32];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
@@ -380,51 +422,45 @@ __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArg
 #pragma unroll
     for (int t = 0; t < L::VT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-  char* vt = lds + wave * L::V_BYTES;
 
-  for (int k0 = begin + wave * kTurn; k0 < end; k0 += 4 * kTurn) {
-    const int last = n.k - 1;
-    v8 kf[2][2][D / 32];
+  for (; k0 < end; k0 += 4 * kTurn) {
+    const int next = k0 + 4 * kTurn;
+    wait_copies<L::V_COPIES>();                                          // K is here, V may be on its way
+    f32x4 s[2][2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const T* kr = k + (int64_t)min(k0 + 16 * j + (lane & 15), last) * a.ks[1] + 8 * g;
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int j = 0; j < 2; ++j) {
+        s[i][j] = f32x4{0, 0, 0, 0};
+        const int r = lane & 15;
 #pragma unroll
-        for (int u = 0; u < D / 32; ++u) kf[i][j][u] = *reinterpret_cast<const v8*>(kr + i * a.ks[2] + 32 * u);
-    }
-#pragma unroll
-    for (int u = 0; u < L::V_BYTES / 1024; ++u) {
-      const int p = u * 64 + lane, row = p / L::VP, pos = p % L::VP;
-      glds16(v + (int64_t)min(k0 + row, last) * a.vs[1] + 8 * (pos ^ L::v_swizzle(row)), vt + u * 1024);
-    }
+        for (int u = 0; u < D / 32; ++u) {
+          const v8 kf = *reinterpret_cast<const v8*>(kt + ((i * kTurn + 16 * j + r) * L::KP + ((4 * u + g) ^ L::k_swizzle(r))) * 16);
+          s[i][j] = Mat<T>::mma16(kf, qf[i][u], s[i][j]);
+        }
+      }
+    wait_reads();
+    if (next < end) request_k<T, D>(a, k + (int64_t)next * a.ks[1], n.k - 1 - next, kt_at);
     v8 pf[2];
     const bool part = k0 + kTurn > full;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      f32x4 s[2];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        s[j] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int u = 0; u < D / 32; ++u) s[j] = Mat<T>::mma16(kf[i][j][u], qf[i][u], s[j]);
-      }
-      if (part || k0 + kTurn > end) {
+      if (part) {
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int key = k0 + 16 * j + 4 * g + e;
-            bool seen = key < limit && key < end;
+            bool seen = key < limit;
             if (mask) seen = seen && mask[(int64_t)min(key, a.k_len - 1) * a.ms[3]];
-            s[j][e] = seen ? s[j][e] : -INFINITY;
+            s[i][j][e] = seen ? s[i][j][e] : -INFINITY;
           }
       }
-      float top = s[0][0];
+      float top = s[i][0][0];
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, s[j][e]);
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, s[i][j][e]);
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       if (__any(top > m[i])) {
@@ -439,36 +475,40 @@ __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArg
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = exp2_(fmaf(s[j][e], a.c, -mc));
+          const float p = exp2_(fmaf(s[i][j][e], a.c, -mc));
           l[i] += p;
           pf[i][4 * j + e] = (T)p;
         }
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                     // V has landed (this wave's own copies: no barrier)
+    if (next < end) wait_copies<L::K_COPIES>();                          // V is here, the next K may be on its way
+    else wait_copies<0>();
     if (part) {                                                          // infinities and NaN that a row does not see (see quarantine above)
       auto finite16 = [](unsigned short u) { return std::is_same<T, bf16>::value ? (u & 0x7f80) != 0x7f80 : (u & 0x7c00) != 0x7c00; };
       bool bad = false;
-      for (int p = lane; p < L::V_BYTES / 2; p += 64) bad |= !finite16(reinterpret_cast<const unsigned short*>(vt)[p]);
+      for (int p = lane; p < L::V_COPIES * 512; p += 64) bad |= !finite16(reinterpret_cast<const unsigned short*>(vt)[p]);
       if (__any(bad)) {
         for (int key = 0; key < kTurn; ++key) {
-          const bool seen = k0 + key < limit && k0 + key < end && (!mask || mask[(int64_t)(k0 + key) * a.ms[3]]);
+          const bool seen = k0 + key < limit && (!mask || mask[(int64_t)(k0 + key) * a.ms[3]]);
+          int gg = g;
+          asm volatile("" : "+v"(gg));                                   // (addresses computed here, not kept from the loop's head)
 #pragma unroll
           for (int t = 0; t < L::VT; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int dv = 16 * t + 4 * g + e;
+              const int dv = 16 * t + 4 * gg + e;
               const T val = reinterpret_cast<const T*>(vt + key * L::VP * 16)[8 * ((dv / 8) ^ L::v_swizzle(key)) + dv % 8];
               if (seen && !finite16(__builtin_bit_cast(unsigned short, val))) { acc[0][t][e] += (float)val; acc[1][t][e] += (float)val; }
             }
         }
-        THA4_WAVE_SYNC();
-        for (int p = lane; p < L::V_BYTES / 2; p += 64) {
+        wait_reads();
+        for (int p = lane; p < L::V_COPIES * 512; p += 64) {
           unsigned short* u = reinterpret_cast<unsigned short*>(vt) + p;
           if (!finite16(*u)) *u = 0;
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        wait_reads();
       }
     }
+    // k slot (g, e) of the product holds key 16 (e / 4) + 4 g + e % 4: the accumulator layout of the two tiles of S^T
 #pragma unroll
     for (int t = 0; t < L::VT; ++t) {
       const int r0 = 4 * g + ((lane & 15) >> 2), piece = 2 * t + ((lane & 3) >> 1), in = 8 * (lane & 1);
@@ -478,7 +518,8 @@ __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArg
       acc[0][t] = Mat<T>::mma16(vf, pf[0], acc[0][t]);
       acc[1][t] = Mat<T>::mma16(vf, pf[1], acc[1][t]);
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                   // the next turn's copies overwrite what was read here
+    wait_reads();
+    if (next < end) request_v<T, D>(a, v + (int64_t)next * a.vs[1], n.k - 1 - next, vt_at);
   }
 
   // the four waves meet: common maxima, then two rounds of sums
@@ -526,44 +567,74 @@ __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArg
     finish_few<T, D>(a, acc, S[0], S[1], b, kv, R, rows, n.q);
     return;
   }
-  float* part = a.work + ((((int64_t)b * a.kv_heads + kv) * a.row_tiles + rt) * a.splits + split) * L::PART;
+  if (R >= rows) return;
+  float* part = a.work + (((int64_t)tile * a.part_rows + (lane & 15)) * a.splits + split) * L::PART;
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int t = 0; t < L::VT; ++t) reinterpret_cast<f32x4*>(part)[(i * L::VT + t) * 64 + lane] = acc[i][t];
-    if (lane < kRows) { part[L::SET + 2 * i * kRows + lane] = M[i]; part[L::SET + (2 * i + 1) * kRows + lane] = S[i]; }
-  }
+    for (int t = 0; t < L::VT; ++t) *reinterpret_cast<f32x4*>(part + i * 2 * D + 16 * t + 4 * g) = acc[i][t];
+  if (g == 0) *reinterpret_cast<f32x4*>(part + 4 * D) = f32x4{M[0], S[0], M[1], S[1]};
 }
 
-// joins the ranges of the keys: the same rescaled sum over the ranges that hold keys, in their order
+// Joins the ranges of the keys: a workgroup for each query and head, the same rescaled sums over the ranges that hold keys.  512 threads: 16-byte pieces of O1 and O2
+// side by side, 512 / D ranges at a time (one workgroup reads the parts of one row only: with few rows the parts are what takes the time).
 template <class T, int D>
-__global__ void __launch_bounds__(64) diff_join_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(512) diff_join_kernel(AttnArgs a) {
   warm_kernarg<(int)sizeof(AttnArgs)>();
   typedef Few<D> L;
-  const int lane = threadIdx.x;
-  int id = blockIdx.x;
-  const int rt = id % a.row_tiles; id /= a.row_tiles;
+  constexpr int SIDE = 512 / D;
+  __shared__ float stat[4][kMaxSplits];                                  // m1, l1, m2, l2 of each range
+  __shared__ f32x4 sum[SIDE][D];
+  const int lane = threadIdx.x & 63;
+  const int row = blockIdx.x % a.part_rows, tile = blockIdx.x / a.part_rows;
+  int id = tile;
+  const int R = (id % a.row_tiles) * kRows + row; id /= a.row_tiles;
   const int kv = id % a.kv_heads, b = id / a.kv_heads;
+  if (R >= a.q_len * a.group) return;
+  const int head = kv * a.group + R % a.group, qi = R / a.group;
   const Lengths n = lengths_of(a, b);
+  if (qi >= n.q) return;
   const int used = (n.k + a.chunk - 1) / a.chunk;
-  const float* part = a.work + (((int64_t)b * a.kv_heads + kv) * a.row_tiles + rt) * a.splits * L::PART;
-  f32x4 acc[2][L::VT];
+  const float* part = a.work + ((int64_t)tile * a.part_rows + row) * a.splits * L::PART;
+  for (int s = threadIdx.x; s < used; s += 512) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(part + (int64_t)s * L::PART + 4 * D);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) stat[i][s] = v[i];
+  }
+  const int slot = threadIdx.x % D, side = threadIdx.x / D, map = slot / (D / 2);
+  __syncthreads();
   float M[2] = {-INFINITY, -INFINITY}, S[2] = {0.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-#pragma unroll
-    for (int t = 0; t < L::VT; ++t) acc[i][t] = f32x4{0, 0, 0, 0};
-    for (int s = 0; s < used; ++s) M[i] = fmaxf(M[i], part[s * L::PART + L::SET + 2 * i * kRows + (lane & 15)]);
-    for (int s = 0; s < used; ++s) {
-      const float* p = part + (int64_t)s * L::PART;
-      const float m = p[L::SET + 2 * i * kRows + (lane & 15)], l = p[L::SET + (2 * i + 1) * kRows + (lane & 15)];
-      const float w = m == -INFINITY ? 1.0f : exp2_((m - M[i]) * a.c);
-      S[i] += l * w;
-#pragma unroll
-      for (int t = 0; t < L::VT; ++t) acc[i][t] += w * reinterpret_cast<const f32x4*>(p)[(i * L::VT + t) * 64 + lane];
-    }
+    for (int s = lane; s < used; s += 64) M[i] = fmaxf(M[i], stat[2 * i][s]);
+    M[i] = wave_reduce(M[i], MaxAbs());
+    for (int s = lane; s < used; s += 64) S[i] += stat[2 * i][s] == -INFINITY ? stat[2 * i + 1][s] : stat[2 * i + 1][s] * exp2_((stat[2 * i][s] - M[i]) * a.c);
+    S[i] = wave_reduce(S[i], Add());
   }
-  finish_few<T, D>(a, acc, S[0], S[1], b, kv, rt * kRows + lane % 16, a.q_len * a.group, n.q);
+  f32x4 acc = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int s = side; s < used; s += SIDE) {
+    const float m = stat[2 * map][s], w = m == -INFINITY ? 1.0f : exp2_((m - (map ? M[1] : M[0])) * a.c);
+    acc += w * *reinterpret_cast<const f32x4*>(part + (int64_t)s * L::PART + 4 * slot);
+  }
+  sum[side][slot] = acc;
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  const float lam = lambda_of<D>(a, head);
+  const int at = min(lane, D / 2 - 1);
+  f32x4 o[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    o[i] = sum[0][i * (D / 2) + at];
+#pragma unroll
+    for (int s = 1; s < SIDE; ++s) o[i] += sum[s][i * (D / 2) + at];
+  }
+  o[0] = o[0] * weight_of(1.0f, S[0]) - o[1] * weight_of(lam, S[1]);
+  float ss = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) ss = fmaf(o[0][e], o[0][e], ss);
+  ss = wave_reduce(lane < D / 2 ? ss : 0.0f, Add());
+  if (lane < D / 2) store_columns<T, D>(a, static_cast<T*>(a.out) + b * a.os[0] + qi * a.os[1] + head * a.os[2], 4 * lane, o[0], norm_factor<D>(a, ss));
 }
 
 }  // namespace xf

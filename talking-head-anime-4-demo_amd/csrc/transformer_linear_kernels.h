@@ -107,11 +107,12 @@ __global__ void __launch_bounds__(256) quantize_any_kernel(QuantArgs a) {
 
 // ---- product -----------------------------------------------------------------------------------------------------------------------------
 struct LinearArgs {
-  const int8_t *x, *w;
+  const void* x;               // int8 [m][k], or (linear_token_kernel) the float tokens themselves
+  const int8_t* w;
   const float *xs, *ws, *bias;
   void* y;
   int64_t m, n, k, x_stride, w_stride, y_stride;
-  int32_t y_dtype;
+  int32_t x_dtype, y_dtype;
 };
 
 THA4_DEV void store_y(void* y, int dtype, int64_t at, float v) {
@@ -137,13 +138,19 @@ THA4_DEV i32x4 piece16(const int8_t* p, int64_t k, int64_t n) {
   return v;
 }
 
-// Few tokens: the weights are the traffic.  A workgroup owns 16 channels x 16 MT tokens; its 8 waves take turns of 128 k, weights straight from memory into matrix-instruction
-// operands (nothing else would reuse them), and their exact partial sums meet in LDS.
-template <int MT, bool ALIGNED>
+// Few tokens: the weights are the traffic.  A workgroup owns 16 channels x 16 MT tokens; its 8 waves take turns of 128 k, weights straight from memory into
+// matrix-instruction operands (nothing else would reuse them), AHEAD turns of them requested before the first is used, and their exact partial sums meet in LDS.
+// INLINE: x is float (XT) and at most kInlineTokens x kInlineK: every workgroup quantises the tokens itself, into LDS, while its first weights are on their
+// way - a few hundred instructions against a launch of their own.
+constexpr int kInlineTokens = 4, kInlineBytes = 32768;
+
+template <class XT, int MT, bool ALIGNED, bool INLINE>
 __global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
   warm_kernarg<(int)sizeof(LinearArgs)>();
-  constexpr int WAVES = 8;
+  constexpr int WAVES = 8, AHEAD = MT == 1 ? 4 : 2;
   __shared__ i32x4 part[WAVES][MT][64];
+  __shared__ __attribute__((aligned(16))) int8_t xq[INLINE ? kInlineBytes : 16];
+  __shared__ float xscale[INLINE ? kInlineTokens : 1], slot[WAVES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 15, g = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * (16 * MT);
@@ -155,23 +162,45 @@ __global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
   for (int i = 0; i < MT; ++i) {
     const int64_t row = m0 + 16 * i + r;
     xk[i] = row < a.m ? a.k : 0;                                            // a token behind the last: zeros, nothing is read
-    x[i] = a.x + (row < a.m ? row : 0) * a.x_stride;
+    x[i] = INLINE ? xq + (row < a.m ? row : 0) * a.k : static_cast<const int8_t*>(a.x) + (row < a.m ? row : 0) * a.x_stride;
   }
   i32x4 acc[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) acc[i] = i32x4{0, 0, 0, 0};
-  for (int64_t k0 = wave * 128; k0 < a.k; k0 += WAVES * 128) {
-    i32x4 wf[2], xf[2][MT];
+  i32x4 wf[AHEAD][2];
+  auto weights = [&](int64_t k0) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      wf[s] = piece16<ALIGNED>(w, k0 + 64 * s + 16 * g, a.k);
+    for (int t = 0; t < AHEAD; ++t)
 #pragma unroll
-      for (int i = 0; i < MT; ++i) xf[s][i] = piece16<ALIGNED>(x[i], k0 + 64 * s + 16 * g, xk[i]);
+      for (int s = 0; s < 2; ++s) wf[t][s] = piece16<ALIGNED>(w, k0 + t * (WAVES * 128) + 64 * s + 16 * g, a.k);
+  };
+  weights(wave * 128);
+  if constexpr (INLINE) {
+    for (int row = 0; row < a.m; ++row) {
+      const XT* from = static_cast<const XT*>(a.x) + row * a.x_stride;
+      float m = 0.0f;
+      for (int c = threadIdx.x; c < a.k; c += 512) m = MaxU32()(m, abs_bits((float)from[c]));
+      const Step k = make_step(row_reduce<WAVES>(m, MaxU32(), slot, wave));
+      if (threadIdx.x == 0) xscale[row] = k.scale;
+      for (int c = threadIdx.x; c < a.k; c += 512) xq[row * a.k + c] = (int8_t)quantize1((float)from[c], k);
+      __syncthreads();                                                      // (slot is free again; after the last row: everything is there)
     }
+  }
+  for (int64_t k0 = wave * 128; k0 < a.k; k0 += AHEAD * WAVES * 128) {
+    i32x4 xf[AHEAD][2][MT];
 #pragma unroll
-    for (int s = 0; s < 2; ++s)
+    for (int t = 0; t < AHEAD; ++t)
 #pragma unroll
-      for (int i = 0; i < MT; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[s], xf[s][i], acc[i], 0, 0, 0);
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) xf[t][s][i] = piece16<ALIGNED>(x[i], k0 + t * (WAVES * 128) + 64 * s + 16 * g, xk[i]);
+#pragma unroll
+    for (int t = 0; t < AHEAD; ++t)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[t][s], xf[t][s][i], acc[i], 0, 0, 0);
+    weights(k0 + AHEAD * WAVES * 128);                                      // (behind the row's end: zeros, nothing is read)
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i) part[wave][i][lane] = acc[i];
@@ -183,7 +212,7 @@ __global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
     for (int v = 1; v < WAVES; ++v) s += part[v][i][l];
     const int64_t row = m0 + 16 * i + (l & 15);
     if (row >= a.m) continue;
-    const float xs = a.xs[row];
+    const float xs = INLINE ? xscale[row] : a.xs[row];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int64_t col = n0 + 4 * (l >> 4) + e;
@@ -195,65 +224,135 @@ __global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
   }
 }
 
-// Many tokens: 128 x 128 outputs a workgroup, four waves of 64 x 64 (2 x 2 matrix tiles of 32 x 32), operands through LDS in steps of 64 k.
-// 16-byte pieces of a row are permuted by (row / 4) mod 4, so that the 16 lanes the LDS serves together hit 16 different 16-byte slots.
-template <bool ALIGNED>
-__global__ void __launch_bounds__(256) linear_tile_kernel(LinearArgs a) {
+// Many tokens: BM tokens x BN channels a workgroup of WM x WN waves, operands through LDS in stages of 64 k.
+//  * 16-byte pieces of a row are permuted by (row / 4) mod 4, so that the 16 lanes the LDS serves together hit 16 different 16-byte slots.
+//  * DMA (aligned rows): STAGES stages of LDS, filled by asynchronous copies two or three stages ahead behind counted waits - one barrier a stage, which both
+//    publishes the stage and frees the one read before.  Otherwise rows go through registers, one stage ahead.
+//  * Channels are the matrix tile's rows, dealt so that a lane ends with 16 consecutive channels of one token: the result leaves in 16-byte stores.
+__device__ const i32x4 g_zero16 = {0, 0, 0, 0};                              // what a copy reads behind a row's end
+
+template <int BM, int BN, int WM, int WN, int STAGES, bool DMA>
+__global__ void __launch_bounds__(64 * WM * WN) linear_tile_kernel(LinearArgs a) {
   warm_kernarg<(int)sizeof(LinearArgs)>();
-  constexpr int BM = 128, BN = 128, BK = 64;
-  __shared__ __attribute__((aligned(16))) char lx[BM * BK], lw[BN * BK];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t m0 = (int64_t)blockIdx.y * BM, n0 = (int64_t)blockIdx.x * BN;
-  const int wm = (wave & 1) * 64, wn = (wave >> 1) * 64;
-  i32x16 acc[2][2];
+  constexpr int WAVES = WM * WN, BK = 64, FM = BM / WM / 32, FN = BN / WN / 32;      // 32 x 32 tiles of a wave
+  constexpr int STAGE = (BM + BN) * BK, PIECES = STAGE / 1024 / WAVES;               // 1-KiB copies of a wave and stage
+  static_assert(PIECES * WAVES * 1024 == STAGE && (BM * BK / 1024) % WAVES == 0, "a copy moves rows of one operand");
+  __shared__ __attribute__((aligned(16))) char lds[(DMA ? STAGES : 1) * STAGE];
+  const int lane = threadIdx.x & 63, wave = uniform_i32(threadIdx.x >> 6), h = lane >> 5;
+  // tiles of one band of tokens run next to each other; blockIdx.x goes round the eight XCDs, so each takes a contiguous eighth of the order
+  const int tiles_n = (int)((a.n + BN - 1) / BN), tiles = (int)gridDim.x;
+  int id = blockIdx.x;
+  const int even = tiles / 8 * 8;
+  if (id < even) id = (id % 8) * (even / 8) + id / 8;
+  const int64_t m0 = (int64_t)(id / tiles_n) * BM, n0 = (int64_t)(id % tiles_n) * BN;
+  const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
+
+  // this lane's place in each copy: 16 rows of 4 pieces a KiB
+  const int8_t* from[PIECES];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int u = 0; u < PIECES; ++u) {
+    const int row = (u * WAVES + wave) * 16 + lane / 4;
+    const int64_t rx = m0 + row < a.m ? m0 + row : a.m - 1, rw = n0 + row - BM < a.n ? n0 + row - BM : a.n - 1;
+    from[u] = u * WAVES * 16 < BM ? static_cast<const int8_t*>(a.x) + rx * a.x_stride : a.w + rw * a.w_stride;
+  }
+  const int piece = 16 * ((lane % 4) ^ ((lane / 16) & 3));                             // (row / 4) mod 4 = (lane / 16): copies start at multiples of 16 rows
+  const int stages = (int)((a.k + BK - 1) / BK);
+
+  i32x16 acc[FN][FM];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = i32x16{0};
-  for (int64_t k0 = 0; k0 < a.k; k0 += BK) {
-    i32x4 fx[2], fw[2];
+  for (int i = 0; i < FN; ++i)
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int id = threadIdx.x + 256 * u, row = id >> 2, p = (id & 3) ^ ((row >> 2) & 3);
-      const int64_t rx = m0 + row < a.m ? m0 + row : a.m - 1, rw = n0 + row < a.n ? n0 + row : a.n - 1;
-      fx[u] = piece16<ALIGNED>(a.x + rx * a.x_stride, k0 + 16 * p, a.k);
-      fw[u] = piece16<ALIGNED>(a.w + rw * a.w_stride, k0 + 16 * p, a.k);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      *reinterpret_cast<i32x4*>(lx + 16 * (threadIdx.x + 256 * u)) = fx[u];
-      *reinterpret_cast<i32x4*>(lw + 16 * (threadIdx.x + 256 * u)) = fw[u];
-    }
-    __syncthreads();
+    for (int j = 0; j < FM; ++j) acc[i][j] = i32x16{0};
+  const int ch = 16 * ((lane >> 2) & 1) + 4 * ((lane & 31) >> 3) + (lane & 3);         // row of the matrix tile -> channel
+  auto compute = [&](const char* stage) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      i32x4 xf[2], wf[2];
-      const int c = 2 * s + (lane >> 5);
+      i32x4 xf[FM], wf[FN];
+      const int c = 2 * s + h;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int rx = wm + 32 * i + (lane & 31), rw = wn + 32 * i + (lane & 31);
-        xf[i] = *reinterpret_cast<const i32x4*>(lx + rx * BK + 16 * (c ^ ((rx >> 2) & 3)));
-        wf[i] = *reinterpret_cast<const i32x4*>(lw + rw * BK + 16 * (c ^ ((rw >> 2) & 3)));
+      for (int j = 0; j < FM; ++j) {
+        const int row = wm + 32 * j + (lane & 31);
+        xf[j] = *reinterpret_cast<const i32x4*>(stage + row * BK + 16 * (c ^ ((row >> 2) & 3)));
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < FN; ++i) {
+        const int row = wn + 32 * i + ch;
+        wf[i] = *reinterpret_cast<const i32x4*>(stage + (BM + row) * BK + 16 * (c ^ ((row >> 2) & 3)));
+      }
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(xf[i], wf[j], acc[i][j], 0, 0, 0);
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[i], xf[j], acc[i][j], 0, 0, 0);
+    }
+  };
+
+  if constexpr (DMA) {
+    const unsigned base = lds_address(lds);
+    auto request = [&](int t) {
+      const int64_t at = (int64_t)t * BK + piece;
+#pragma unroll
+      for (int u = 0; u < PIECES; ++u)
+        copy16_async(at < a.k ? (const void*)(from[u] + at) : (const void*)&g_zero16, base + (t % STAGES) * STAGE + (u * WAVES + wave) * 1024);
+    };
+#pragma unroll
+    for (int t = 0; t < STAGES - 1; ++t)
+      if (t < stages) request(t);
+    for (int t = 0; t < stages; ++t) {
+      const int newer = min(stages - 1 - t, STAGES - 2);                               // stages requested behind this one
+      THA4_BARRIER_KEEP(newer * PIECES);                                               // (and this wave's own reads of the stage before are done)
+      if (t + STAGES - 1 < stages) request(t + STAGES - 1);                            // into the stage everybody finished in front of the barrier
+      compute(lds + (t % STAGES) * STAGE);
+    }
+  } else {
+    i32x4 hold[PIECES];
+    auto request = [&](int t) {
+#pragma unroll
+      for (int u = 0; u < PIECES; ++u) hold[u] = piece16<false>(from[u], (int64_t)t * BK + piece, a.k);
+    };
+    request(0);
+    for (int t = 0; t < stages; ++t) {
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < PIECES; ++u) *reinterpret_cast<i32x4*>(lds + (u * WAVES + wave) * 1024 + 16 * lane) = hold[u];
+      __syncthreads();
+      if (t + 1 < stages) request(t + 1);
+      compute(lds);
     }
   }
+
+  const bool vec = a.n % 8 == 0 && a.y_stride % 8 == 0 && (reinterpret_cast<size_t>(a.y) & 15) == 0;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int64_t col = n0 + wn + 32 * j + (lane & 31);
-    if (col >= a.n) continue;
-    const float ws = a.ws[col], b = a.bias ? a.bias[col] : 0.0f;
+  for (int i = 0; i < FN; ++i) {
+    const int64_t col = n0 + wn + 32 * i + 16 * h;
+    float ws[16], b[16];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int e = 0; e < 16; ++e) {
+      const int64_t c = col + e < a.n ? col + e : a.n - 1;
+      ws[e] = a.ws[c];
+      b[e] = a.bias ? a.bias[c] : 0.0f;
+    }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int64_t row = m0 + wm + 32 * i + 8 * (e / 4) + 4 * (lane >> 5) + e % 4;
-        if (row < a.m) store_y(a.y, a.y_dtype, row * a.y_stride + col, (float)acc[i][j][e] * a.xs[row] * ws + b);
+    for (int j = 0; j < FM; ++j) {
+      const int64_t row = m0 + wm + 32 * j + (lane & 31);
+      if (row >= a.m) continue;
+      const float xs = a.xs[row];
+#pragma unroll
+      for (int o = 0; o < 16; o += 8) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = fmaf((float)acc[i][j][o + e] * xs, ws[o + e], b[o + e]);
+        const int64_t at = row * a.y_stride + col + o;
+        if (vec && col + o < a.n) {
+          if (a.y_dtype == 0) put8(static_cast<float*>(a.y) + at, v);
+          else if (a.y_dtype == 1) put8(static_cast<f16*>(a.y) + at, v);
+          else put8(static_cast<bf16*>(a.y) + at, v);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (col + o + e < a.n) store_y(a.y, a.y_dtype, at + e, v[e]);
+        }
       }
+    }
   }
 }
 

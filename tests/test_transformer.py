@@ -41,7 +41,7 @@ def test_quantize_refuses(lib):
 
 
 def linear_args(p, **more):
-    a = dict(x_dev=p, x_scale_dev=p, w_dev=p, w_scale_dev=p, bias_dev=None, y_dev=p, m=1, n=1, k=1, x_row_stride=1, w_row_stride=1, y_row_stride=1, y_dtype=0)
+    a = dict(x_dev=p, x_scale_dev=p, w_dev=p, w_scale_dev=p, bias_dev=None, y_dev=p, m=1, n=1, k=1, x_row_stride=1, w_row_stride=1, y_row_stride=1, x_dtype=3, y_dtype=0)
     a.update(more)
     return C.byref(_capi.Tha4LinearI8Args(**{n: v.value if isinstance(v, C.c_void_p) else v for n, v in a.items()}))
 
@@ -50,7 +50,13 @@ def test_linear_refuses(lib):
     p, keep = host()
     f = lib.tha4_linear_i8
     refused(lib, f(None, None), "NULL")
+    assert lib.tha4_linear_i8_workspace(None) == -1
     refused(lib, f(linear_args(p, y_dtype=7), None), "y_dtype")
+    refused(lib, f(linear_args(p, x_dtype=4), None), "x_dtype")
+    refused(lib, lib.tha4_linear_i8_workspace(linear_args(p, x_dtype=4)), "x_dtype")
+    refused(lib, f(linear_args(p, x_scale_dev=None), None), "x_scale")
+    refused(lib, f(linear_args(p, x_dtype=2), None), "x_scale")
+    refused(lib, f(linear_args(p, x_dtype=2, x_scale_dev=None, m=100, k=64, x_row_stride=64), None), "workspace")
     refused(lib, f(linear_args(p, k=0), None), "k must be positive")
     refused(lib, f(linear_args(p, m=-1), None), "negative")
     refused(lib, f(linear_args(p, k=131072), None), "131071")
@@ -151,8 +157,6 @@ def test_python_refuses_cpu_tensors_and_wrong_shapes(lib):
         transformer.residual_norm(x, torch.zeros(3, 32))
     with pytest.raises(AssertionError, match="post_norm"):
         transformer.residual_norm(x, x, post_norm="batch")
-    with pytest.raises(AssertionError, match="all be float32"):
-        transformer.residual_norm(x, x, pre_weight=torch.ones(32), post_weight=torch.ones(32, dtype=torch.bfloat16))
     q = torch.zeros(1, 3, 4, 32, dtype=torch.bfloat16)
     v = torch.zeros(1, 3, 2, 64, dtype=torch.bfloat16)
     lam = torch.zeros(4, 32)

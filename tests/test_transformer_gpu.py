@@ -481,8 +481,17 @@ def test_refusals_on_the_device():
         transformer.residual_norm(x.clone().requires_grad_())
     with torch.no_grad():
         transformer.residual_norm(x.clone().requires_grad_())
-    with pytest.raises(AssertionError, match="must be on the GPU"):
+    with pytest.raises(AssertionError, match="on one GPU"):
         transformer.residual_norm(x, x, post_weight=torch.ones(64))
+    one = torch.ones(64, device="cuda:0")
+    with pytest.raises(AssertionError, match="all be float32"):
+        transformer.residual_norm(x, x, pre_weight=one, post_weight=one.to(BF16))
+    with pytest.raises(AssertionError, match="all be float32"):
+        transformer.residual_norm(x, x, pre_weight=one, film=(one.half(), one.half()))
+    with pytest.raises(AssertionError, match="vectors"):
+        transformer.residual_norm(x, x, pre_weight=one[:1])
+    with pytest.raises(AssertionError, match="one row"):
+        transformer.residual_norm(torch.zeros(4, 6, 64, device="cuda:0"), torch.zeros(4, 6, 64, device="cuda:0"), gate=torch.zeros(3, 64, device="cuda:0"))
     with pytest.raises(AssertionError, match="x_scale"):
         transformer.int8_linear(x.to(torch.int8), torch.zeros(4, 64, dtype=torch.int8, device="cuda:0"), torch.ones(4, device="cuda:0"))
     with pytest.raises(_capi.Tha4Error, match="131071"):
