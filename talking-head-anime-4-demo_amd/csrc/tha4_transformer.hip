@@ -78,18 +78,23 @@ int few(const LinearArgs& a, bool al, void* stream) {
   const int64_t nb = ceil_div(a.n, 16), mb = ceil_div(a.m, 16 * MT);
   return al ? launch(linear_few_kernel<XT, MT, true, INLINE>, nb, mb, 512, a, stream) : launch(linear_few_kernel<XT, MT, false, INLINE>, nb, mb, 512, a, stream);
 }
-template <int BM, int BN, int WM, int WN, int STAGES>
+template <int BM, int BN, int WM, int WN, int G, int STAGES>
 int tile(const LinearArgs& a, bool al, void* stream) {
   const int64_t tiles = ceil_div(a.m, BM) * ceil_div(a.n, BN);
-  return al ? launch(linear_tile_kernel<BM, BN, WM, WN, STAGES, true>, tiles, 1, 64 * WM * WN, a, stream)
-            : launch(linear_tile_kernel<BM, BN, WM, WN, STAGES, false>, tiles, 1, 64 * WM * WN, a, stream);
+  return al ? launch(linear_tile_kernel<BM, BN, 128, WM, WN, G, STAGES, true>, tiles, 1, 64 * WM * WN * G, a, stream)
+            : launch(linear_tile_kernel<BM, BN, 128, WM, WN, G, STAGES, false>, tiles, 1, 64 * WM * WN * G, a, stream);
 }
+// Which kernel: by the number of tokens, then the largest tile whose grid still covers most of the 256 CUs (us, w one of three in turn, bf16 out):
+//   m <= 32  weights straight into operands      32 x 4096 x 4096: 11.2 against 13.7 on 64 x 64 tiles;  64 x 8192 x 8192: 40.2 against 20.8 - tiles from 33 tokens on
+//   256 x 256 from 192 tiles on                  8192^3: 531 against 781 on 128 x 128
+//   64 x 64 at most 256 tiles: four groups       256 x 4096 x 4096: 12.2 against 14.9 with one group;  320 x 4096 x 4096 (320 tiles): 22.9 against 17.0
 int product(const LinearArgs& a, bool al, void* stream) {
   if (a.m <= 16) return few<float, 1, false>(a, al, stream);
-  if (a.m <= 64) return few<float, 4, false>(a, al, stream);
-  if (al && ceil_div(a.m, 256) * ceil_div(a.n, 256) >= 192) return tile<256, 256, 2, 4, 4>(a, al, stream);
-  if (ceil_div(a.m, 128) * ceil_div(a.n, 128) >= 192) return tile<128, 128, 2, 2, 4>(a, al, stream);
-  return tile<64, 64, 2, 2, 4>(a, al, stream);
+  if (a.m <= 32) return few<float, 2, false>(a, al, stream);
+  if (ceil_div(a.m, 256) * ceil_div(a.n, 256) >= 192) return tile<256, 256, 4, 2, 1, 2>(a, al, stream);
+  if (ceil_div(a.m, 128) * ceil_div(a.n, 128) >= 192) return tile<128, 128, 2, 2, 1, 2>(a, al, stream);
+  if (ceil_div(a.m, 64) * ceil_div(a.n, 64) > 256) return tile<64, 64, 2, 2, 1, 4>(a, al, stream);
+  return tile<64, 64, 2, 2, 4, 2>(a, al, stream);
 }
 
 // ---- norms ----
@@ -119,7 +124,10 @@ Plan plan_of(const tha4_diff_attention_args& a) {
   p.row_tiles = (int)ceil_div(rows, kRows);
   p.part_rows = (int)std::min<int64_t>(rows, kRows);
   const int64_t wgs = std::max<int64_t>((int64_t)a.batch * a.kv_heads * p.row_tiles, 1);
-  const int64_t want = std::min<int64_t>(ceil_div(a.kv_lengths_dev ? 2048 : 1024, wgs), kMaxSplits);
+  // Workgroups to aim for.  Full caches: what the GPU holds at once (256 CUs, one workgroup each at d = 128, two below; 131072 keys, d = 128, 8 heads on 2: 256 -> 63 us, 512 ->
+  // 71 us, 1024 -> 90 us: the parts to join grow).  Caches of their own lengths: many more, for the short ones end at once (32 x 16384 keys: 512 -> 138 us, 1024 -> 146 us, 2048 -> 131 us, 8192 -> 132 us).
+  const int64_t aim = a.kv_lengths_dev ? 2048 : a.head_dim == 128 ? 256 : 512;
+  const int64_t want = std::min<int64_t>(ceil_div(aim, wgs), kMaxSplits);
   const int64_t chunk = std::max<int64_t>(ceil_div(ceil_div(a.k_len, want), 128) * 128, 256);
   p.splits = (int)std::max<int64_t>(ceil_div(a.k_len, chunk), 1);
   p.chunk = (int)chunk;

@@ -388,9 +388,10 @@ __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArg
   __shared__ float stat[4][4][kRows];
   const int lane = threadIdx.x & 63, wave = uniform_i32(threadIdx.x >> 6), g = lane >> 4;
   int id = blockIdx.x;
+  // kv heads next to each other: their rows of a token are neighbours in memory (32 x 16384 keys, 4 kv heads, d = 64: 131 -> 122 us against ranges next to each other)
+  const int kv = id % a.kv_heads; id /= a.kv_heads;
   const int split = id % a.splits; id /= a.splits;
-  const int rt = id % a.row_tiles, tile = id; id /= a.row_tiles;
-  const int kv = id % a.kv_heads, b = id / a.kv_heads;
+  const int rt = id % a.row_tiles, b = id / a.row_tiles, tile = (b * a.kv_heads + kv) * a.row_tiles + rt;
   const Lengths n = lengths_of(a, b);
   const int rows = a.q_len * a.group, R = rt * kRows + (lane & 15), Rc = min(R, rows - 1);
   const int qi = min(Rc / a.group, max(n.q - 1, 0)), head = kv * a.group + Rc % a.group;

@@ -48,6 +48,13 @@ THA4_DEV int quantize1(float x, const Step& k) {
   return (int)fminf(fmaxf(q, -127.0f), 127.0f);
 }
 
+THA4_DEV uint2 quantize8(const float (&v)[8], const Step& k) {
+  unsigned w[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e / 4] |= ((unsigned)quantize1(v[e], k) & 255u) << (8 * (e % 4));
+  return make_uint2(w[0], w[1]);
+}
+
 // TPR threads share a row that stays in registers between the maximum and the rounding: read once
 template <class T, int TPR, int NV>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quantize_kernel(QuantArgs a) {
@@ -83,10 +90,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quantize_kernel(QuantAr
     if (c >= a.cols) continue;
     float v[8];
     unpack8(raw[j], v);
-    unsigned w[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w[e / 4] |= ((unsigned)quantize1(v[e], k) & 255u) << (8 * (e % 4));
-    *reinterpret_cast<uint2*>(q + c) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(q + c) = quantize8(v, k);
   }
 }
 
@@ -139,7 +143,7 @@ THA4_DEV i32x4 piece16(const int8_t* p, int64_t k, int64_t n) {
 }
 
 // Few tokens: the weights are the traffic.  A workgroup owns 16 channels x 16 MT tokens; its 8 waves take turns of 128 k, weights straight from memory into
-// matrix-instruction operands (nothing else would reuse them), AHEAD turns of them requested before the first is used, and their exact partial sums meet in LDS.
+// matrix-instruction operands (nothing else would reuse them), AHEAD turns of them on their way at any time, and their exact partial sums meet in LDS.
 // INLINE: x is float (XT) and at most kInlineTokens x kInlineK: every workgroup quantises the tokens itself, into LDS, while its first weights are on their
 // way - a few hundred instructions against a launch of their own.
 constexpr int kInlineTokens = 4, kInlineBytes = 32768;
@@ -154,8 +158,7 @@ __global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 15, g = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * (16 * MT);
-  const int64_t wr = n0 + r < a.n ? n0 + r : a.n - 1;                       // (a channel behind the last: the last again, not stored)
-  const int8_t* w = a.w + wr * a.w_stride;
+  const int8_t* w = a.w + (n0 + r < a.n ? n0 + r : a.n - 1) * a.w_stride;   // (a channel behind the last: the last again, not stored)
   const int8_t* x[MT];
   int64_t xk[MT];
 #pragma unroll
@@ -167,40 +170,58 @@ __global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
   i32x4 acc[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) acc[i] = i32x4{0, 0, 0, 0};
-  i32x4 wf[AHEAD][2];
-  auto weights = [&](int64_t k0) {
+  i32x4 wf[AHEAD][2], xf[AHEAD][2][MT];
+  auto weights = [&](int t, int64_t k0) {                                   // (behind the row's end: zeros, nothing is read)
 #pragma unroll
-    for (int t = 0; t < AHEAD; ++t)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) wf[t][s] = piece16<ALIGNED>(w, k0 + t * (WAVES * 128) + 64 * s + 16 * g, a.k);
+    for (int s = 0; s < 2; ++s) wf[t][s] = piece16<ALIGNED>(w, k0 + 64 * s + 16 * g, a.k);
   };
-  weights(wave * 128);
+  auto tokens = [&](int t, int64_t k0) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) xf[t][s][i] = piece16<ALIGNED>(x[i], k0 + 64 * s + 16 * g, xk[i]);
+  };
+#pragma unroll
+  for (int t = 0; t < AHEAD; ++t) {
+    weights(t, (t * WAVES + wave) * 128);
+    if constexpr (!INLINE) tokens(t, (t * WAVES + wave) * 128);
+  }
   if constexpr (INLINE) {
+    // 16-byte aligned tokens of at most 8 x 512 elements stay in registers between their maximum and their rounding
+    const bool vec = a.k % 8 == 0 && a.k <= 8 * 512 && reinterpret_cast<size_t>(a.x) % 16 == 0 && a.x_stride * sizeof(XT) % 16 == 0;
+    const int c8 = 8 * (int)threadIdx.x;
     for (int row = 0; row < a.m; ++row) {
       const XT* from = static_cast<const XT*>(a.x) + row * a.x_stride;
-      float m = 0.0f;
-      for (int c = threadIdx.x; c < a.k; c += 512) m = MaxU32()(m, abs_bits((float)from[c]));
+      float m = 0.0f, v[8];
+      if (vec) {
+        unpack8(fetch8(from + (c8 < a.k ? c8 : 0)), v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = MaxU32()(m, abs_bits(v[e]));
+      } else {
+        for (int c = threadIdx.x; c < a.k; c += 512) m = MaxU32()(m, abs_bits((float)from[c]));
+      }
       const Step k = make_step(row_reduce<WAVES>(m, MaxU32(), slot, wave));
       if (threadIdx.x == 0) xscale[row] = k.scale;
-      for (int c = threadIdx.x; c < a.k; c += 512) xq[row * a.k + c] = (int8_t)quantize1((float)from[c], k);
+      if (!vec) {
+        for (int c = threadIdx.x; c < a.k; c += 512) xq[row * a.k + c] = (int8_t)quantize1((float)from[c], k);
+      } else if (c8 < a.k) {
+        *reinterpret_cast<uint2*>(xq + row * a.k + c8) = quantize8(v, k);
+      }
       __syncthreads();                                                      // (slot is free again; after the last row: everything is there)
     }
   }
   for (int64_t k0 = wave * 128; k0 < a.k; k0 += AHEAD * WAVES * 128) {
-    i32x4 xf[AHEAD][2][MT];
 #pragma unroll
-    for (int t = 0; t < AHEAD; ++t)
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int i = 0; i < MT; ++i) xf[t][s][i] = piece16<ALIGNED>(x[i], k0 + t * (WAVES * 128) + 64 * s + 16 * g, xk[i]);
-#pragma unroll
-    for (int t = 0; t < AHEAD; ++t)
+    for (int t = 0; t < AHEAD; ++t) {
+      const int64_t at = k0 + t * (WAVES * 128), next = at + AHEAD * WAVES * 128;
+      if constexpr (INLINE) tokens(t, at);
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[t][s], xf[t][s][i], acc[i], 0, 0, 0);
-    weights(k0 + AHEAD * WAVES * 128);                                      // (behind the row's end: zeros, nothing is read)
+      weights(t, next);
+      if constexpr (!INLINE) tokens(t, next);
+    }
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i) part[wave][i][lane] = acc[i];
@@ -224,39 +245,50 @@ __global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
   }
 }
 
-// Many tokens: BM tokens x BN channels a workgroup of WM x WN waves, operands through LDS in stages of 64 k.
-//  * 16-byte pieces of a row are permuted by (row / 4) mod 4, so that the 16 lanes the LDS serves together hit 16 different 16-byte slots.
-//  * DMA (aligned rows): STAGES stages of LDS, filled by asynchronous copies two or three stages ahead behind counted waits - one barrier a stage, which both
-//    publishes the stage and frees the one read before.  Otherwise rows go through registers, one stage ahead.
+// Many tokens: BM tokens x BN channels a workgroup of WM x WN waves (times G groups that take turns along k: where there are few tiles, more of a row is on its way at once), operands through LDS in stages of BK k.
+//  * 16-byte pieces of a row are permuted (swizzle), so that the 16 lanes the LDS serves together hit 16 different 16-byte slots.
+//  * DMA (aligned rows): STAGES stages of LDS, filled by asynchronous copies up to three stages ahead behind counted waits - one barrier a stage, which both
+//    publishes the next stage and frees this one.  Otherwise rows go through registers, one stage ahead.
 //  * Channels are the matrix tile's rows, dealt so that a lane ends with 16 consecutive channels of one token: the result leaves in 16-byte stores.
 __device__ const i32x4 g_zero16 = {0, 0, 0, 0};                              // what a copy reads behind a row's end
 
-template <int BM, int BN, int WM, int WN, int STAGES, bool DMA>
-__global__ void __launch_bounds__(64 * WM * WN) linear_tile_kernel(LinearArgs a) {
+constexpr int kBand = 4;
+
+template <int BM, int BN, int BK, int WM, int WN, int G, int STAGES, bool DMA>
+__global__ void __launch_bounds__(64 * WM * WN * G) linear_tile_kernel(LinearArgs a) {
   warm_kernarg<(int)sizeof(LinearArgs)>();
-  constexpr int WAVES = WM * WN, BK = 64, FM = BM / WM / 32, FN = BN / WN / 32;      // 32 x 32 tiles of a wave
+  constexpr int WAVES = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;      // 32 x 32 tiles of a wave
   constexpr int STAGE = (BM + BN) * BK, PIECES = STAGE / 1024 / WAVES;               // 1-KiB copies of a wave and stage
   static_assert(PIECES * WAVES * 1024 == STAGE && (BM * BK / 1024) % WAVES == 0, "a copy moves rows of one operand");
-  __shared__ __attribute__((aligned(16))) char lds[(DMA ? STAGES : 1) * STAGE];
-  const int lane = threadIdx.x & 63, wave = uniform_i32(threadIdx.x >> 6), h = lane >> 5;
-  // tiles of one band of tokens run next to each other; blockIdx.x goes round the eight XCDs, so each takes a contiguous eighth of the order
-  const int tiles_n = (int)((a.n + BN - 1) / BN), tiles = (int)gridDim.x;
+  constexpr int RING = (DMA ? STAGES : 1) * STAGE;                                    // bytes of one group's stages
+  __shared__ __attribute__((aligned(16))) char lds_all[G * RING];
+  static_assert(G == 1 || (G - 1) * BM * BN * 4 <= G * RING, "the groups' sums meet in the stages");
+  const int lane = threadIdx.x & 63, wave = uniform_i32(threadIdx.x >> 6) % WAVES, group_k = uniform_i32(threadIdx.x >> 6) / WAVES, h = lane >> 5;
+  char* lds = lds_all + group_k * RING;
+  // Order of the tiles: blockIdx.x goes round the eight XCDs, so each gets a contiguous eighth of an order in which kBand bands of tokens run together, column by column: the tiles
+  // an XCD has in flight (32 CUs) form a block of 4 x 8, whose rows of x and w its L2 reads once for all of them (8192^3: 1 band 608 us, 4 bands 579 us, 8 585 us, 16 600 us).
+  const int tiles_n = (int)((a.n + BN - 1) / BN), tiles_m = (int)((a.m + BM - 1) / BM);
   int id = blockIdx.x;
-  const int even = tiles / 8 * 8;
+  const int even = tiles_m * tiles_n / 8 * 8;
   if (id < even) id = (id % 8) * (even / 8) + id / 8;
-  const int64_t m0 = (int64_t)(id / tiles_n) * BM, n0 = (int64_t)(id % tiles_n) * BN;
+  const int group = id / (kBand * tiles_n), bands = min(kBand, tiles_m - group * kBand);
+  id -= group * kBand * tiles_n;
+  const int64_t m0 = (int64_t)(group * kBand + id % bands) * BM, n0 = (int64_t)(id / bands) * BN;
   const int wm = (wave % WM) * (BM / WM), wn = (wave / WM) * (BN / WN);
 
-  // this lane's place in each copy: 16 rows of 4 pieces a KiB
+  // this lane's place in each copy: rows of P 16-byte pieces, 64 pieces a copy
+  constexpr int P = BK / 16;
+  static_assert((P == 4 || P == 8) && WAVES * (64 / P) % 16 == 0, "a 256-byte line of LDS holds four or two rows; a wave's copies lie 16 rows apart or a multiple");
+  auto swizzle = [](int row) { return (row / (16 / P)) & (P - 1); };
   const int8_t* from[PIECES];
 #pragma unroll
   for (int u = 0; u < PIECES; ++u) {
-    const int row = (u * WAVES + wave) * 16 + lane / 4;
+    const int row = (u * WAVES + wave) * (64 / P) + lane / P;
     const int64_t rx = m0 + row < a.m ? m0 + row : a.m - 1, rw = n0 + row - BM < a.n ? n0 + row - BM : a.n - 1;
-    from[u] = u * WAVES * 16 < BM ? static_cast<const int8_t*>(a.x) + rx * a.x_stride : a.w + rw * a.w_stride;
+    from[u] = u * WAVES * (64 / P) < BM ? static_cast<const int8_t*>(a.x) + rx * a.x_stride : a.w + rw * a.w_stride;
   }
-  const int piece = 16 * ((lane % 4) ^ ((lane / 16) & 3));                             // (row / 4) mod 4 = (lane / 16): copies start at multiples of 16 rows
-  const int stages = (int)((a.k + BK - 1) / BK);
+  const int piece = 16 * ((lane % P) ^ swizzle(wave * (64 / P) + lane / P));           // (the permutation repeats after 16 rows: the same in every copy of the wave)
+  const int stages = (int)((a.k + BK * G - 1) / (BK * G));                            // of each group; one behind the row's end is zeros
 
   i32x16 acc[FN][FM];
 #pragma unroll
@@ -264,50 +296,62 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_tile_kernel(LinearArgs a)
 #pragma unroll
     for (int j = 0; j < FM; ++j) acc[i][j] = i32x16{0};
   const int ch = 16 * ((lane >> 2) & 1) + 4 * ((lane & 31) >> 3) + (lane & 3);         // row of the matrix tile -> channel
-  auto compute = [&](const char* stage) {
+  struct Operands { i32x4 x[FM], w[FN]; };
+  auto fetch = [&](const char* stage, int s, Operands& f) {                            // step s (32 k) of a stage
+    const int c = 2 * s + h;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      i32x4 xf[FM], wf[FN];
-      const int c = 2 * s + h;
-#pragma unroll
-      for (int j = 0; j < FM; ++j) {
-        const int row = wm + 32 * j + (lane & 31);
-        xf[j] = *reinterpret_cast<const i32x4*>(stage + row * BK + 16 * (c ^ ((row >> 2) & 3)));
-      }
-#pragma unroll
-      for (int i = 0; i < FN; ++i) {
-        const int row = wn + 32 * i + ch;
-        wf[i] = *reinterpret_cast<const i32x4*>(stage + (BM + row) * BK + 16 * (c ^ ((row >> 2) & 3)));
-      }
-#pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[i], xf[j], acc[i][j], 0, 0, 0);
+    for (int j = 0; j < FM; ++j) {
+      const int row = wm + 32 * j + (lane & 31);
+      f.x[j] = *reinterpret_cast<const i32x4*>(stage + row * BK + 16 * (c ^ swizzle(row)));
     }
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      const int row = wn + 32 * i + ch;
+      f.w[i] = *reinterpret_cast<const i32x4*>(stage + (BM + row) * BK + 16 * (c ^ swizzle(row)));
+    }
+  };
+  auto multiply = [&](const Operands& f) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int j = 0; j < FM; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f.w[i], f.x[j], acc[i][j], 0, 0, 0);
   };
 
   if constexpr (DMA) {
     const unsigned base = lds_address(lds);
     auto request = [&](int t) {
-      const int64_t at = (int64_t)t * BK + piece;
+      const int64_t at = ((int64_t)t * G + group_k) * BK + piece;
 #pragma unroll
       for (int u = 0; u < PIECES; ++u)
         copy16_async(at < a.k ? (const void*)(from[u] + at) : (const void*)&g_zero16, base + (t % STAGES) * STAGE + (u * WAVES + wave) * 1024);
     };
 #pragma unroll
-    for (int t = 0; t < STAGES - 1; ++t)
+    for (int t = 0; t < STAGES; ++t)
       if (t < stages) request(t);
+    THA4_BARRIER_KEEP(min(stages - 1, STAGES - 1) * PIECES);                           // stage 0 is there
+    // Operands of a step are read from LDS under the products of the step before; the barrier that publishes the next stage stands in front of the last products of this one, behind
+    // this wave's last reads of it, so a wave never waits for a barrier and for LDS with nothing to multiply
+    Operands f[2];
+    fetch(lds, 0, f[0]);
     for (int t = 0; t < stages; ++t) {
-      const int newer = min(stages - 1 - t, STAGES - 2);                               // stages requested behind this one
-      THA4_BARRIER_KEEP(newer * PIECES);                                               // (and this wave's own reads of the stage before are done)
-      if (t + STAGES - 1 < stages) request(t + STAGES - 1);                            // into the stage everybody finished in front of the barrier
-      compute(lds + (t % STAGES) * STAGE);
+#pragma unroll
+      for (int u = 0; u < BK / 32; ++u) {
+        if (u + 1 < BK / 32) {
+          fetch(lds + (t % STAGES) * STAGE, u + 1, f[(u + 1) & 1]);
+        } else if (t + 1 < stages) {
+          THA4_BARRIER_KEEP(min(stages - 2 - t, STAGES - 2) * PIECES);
+          if (t + STAGES < stages) request(t + STAGES);                                // into the stage that everybody has read
+          fetch(lds + ((t + 1) % STAGES) * STAGE, 0, f[0]);
+        }
+        THA4_SCHED_FENCE();
+        multiply(f[u & 1]);
+      }
     }
   } else {
     i32x4 hold[PIECES];
     auto request = [&](int t) {
 #pragma unroll
-      for (int u = 0; u < PIECES; ++u) hold[u] = piece16<false>(from[u], (int64_t)t * BK + piece, a.k);
+      for (int u = 0; u < PIECES; ++u) hold[u] = piece16<false>(from[u], ((int64_t)t * G + group_k) * BK + piece, a.k);
     };
     request(0);
     for (int t = 0; t < stages; ++t) {
@@ -316,40 +360,74 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_tile_kernel(LinearArgs a)
       for (int u = 0; u < PIECES; ++u) *reinterpret_cast<i32x4*>(lds + (u * WAVES + wave) * 1024 + 16 * lane) = hold[u];
       __syncthreads();
       if (t + 1 < stages) request(t + 1);
-      compute(lds);
+#pragma unroll
+      for (int u = 0; u < BK / 32; ++u) {
+        Operands f;
+        fetch(lds, u, f);
+        multiply(f);
+      }
     }
   }
 
+  if constexpr (G > 1) {                                                               // integer sums: no order to keep
+    i32x4* meet = reinterpret_cast<i32x4*>(lds_all) + wave * (FN * FM * 4 * 64) + lane;
+    constexpr int SET = WAVES * FN * FM * 4 * 64;
+    __syncthreads();
+    if (group_k) {
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            meet[(group_k - 1) * SET + ((i * FM + j) * 4 + e) * 64] = i32x4{acc[i][j][4 * e], acc[i][j][4 * e + 1], acc[i][j][4 * e + 2], acc[i][j][4 * e + 3]};
+    }
+    __syncthreads();
+    if (group_k) return;
+#pragma unroll
+    for (int v = 0; v < G - 1; ++v)
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const i32x4 o = meet[v * SET + ((i * FM + j) * 4 + e) * 64];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][j][4 * e + r] += o[r];
+            THA4_SCHED_FENCE();
+          }
+  }
   const bool vec = a.n % 8 == 0 && a.y_stride % 8 == 0 && (reinterpret_cast<size_t>(a.y) & 15) == 0;
 #pragma unroll
   for (int i = 0; i < FN; ++i) {
-    const int64_t col = n0 + wn + 32 * i + 16 * h;
-    float ws[16], b[16];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int64_t c = col + e < a.n ? col + e : a.n - 1;
-      ws[e] = a.ws[c];
-      b[e] = a.bias ? a.bias[c] : 0.0f;
-    }
+    for (int o = 0; o < 16; o += 8) {
+      const int64_t col = n0 + wn + 32 * i + 16 * h + o;
+      float ws[8], b[8];
 #pragma unroll
-    for (int j = 0; j < FM; ++j) {
-      const int64_t row = m0 + wm + 32 * j + (lane & 31);
-      if (row >= a.m) continue;
-      const float xs = a.xs[row];
+      for (int e = 0; e < 8; ++e) {
+        const int64_t c = col + e < a.n ? col + e : a.n - 1;
+        ws[e] = a.ws[c];
+        b[e] = a.bias ? a.bias[c] : 0.0f;
+      }
 #pragma unroll
-      for (int o = 0; o < 16; o += 8) {
+      for (int j = 0; j < FM; ++j) {
+        const int64_t row = m0 + wm + 32 * j + (lane & 31);
+        if (row >= a.m) continue;
+        const float xs = a.xs[row];
         float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = fmaf((float)acc[i][j][o + e] * xs, ws[o + e], b[o + e]);
-        const int64_t at = row * a.y_stride + col + o;
-        if (vec && col + o < a.n) {
+        for (int e = 0; e < 8; ++e) v[e] = fmaf((float)acc[i][j][o + e] * xs, ws[e], b[e]);
+        const int64_t at = row * a.y_stride + col;
+        if (vec && col < a.n) {
           if (a.y_dtype == 0) put8(static_cast<float*>(a.y) + at, v);
           else if (a.y_dtype == 1) put8(static_cast<f16*>(a.y) + at, v);
           else put8(static_cast<bf16*>(a.y) + at, v);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (col + o + e < a.n) store_y(a.y, a.y_dtype, at + e, v[e]);
+            if (col + e < a.n) store_y(a.y, a.y_dtype, at + e, v[e]);
         }
       }
     }
