@@ -73,10 +73,12 @@ const char* check_linear(const tha4_linear_i8_args& g) {
 bool inline_tokens(const tha4_linear_i8_args& g) { return g.m <= kInlineTokens && g.m * g.k <= kInlineBytes; }
 int64_t token_stride(const tha4_linear_i8_args& g) { return ceil_div(g.k, 16) * 16; }
 
-template <class XT, int MT, bool INLINE>
+template <class XT, int NT, int MT, bool INLINE>
 int few(const LinearArgs& a, bool al, void* stream) {
-  const int64_t nb = ceil_div(a.n, 16), mb = ceil_div(a.m, 16 * MT);
-  return al ? launch(linear_few_kernel<XT, MT, true, INLINE>, nb, mb, 512, a, stream) : launch(linear_few_kernel<XT, MT, false, INLINE>, nb, mb, 512, a, stream);
+  const int64_t nb = ceil_div(a.n, 16 * NT), mb = ceil_div(a.m, 16 * MT);
+  if constexpr (NT == 1)
+    if (!al) return launch(linear_few_kernel<XT, NT, MT, false, INLINE>, nb, mb, 512, a, stream);
+  return launch(linear_few_kernel<XT, NT, MT, true, INLINE>, nb, mb, 512, a, stream);
 }
 template <int BM, int BN, int WM, int WN, int G, int STAGES>
 int tile(const LinearArgs& a, bool al, void* stream) {
@@ -85,12 +87,13 @@ int tile(const LinearArgs& a, bool al, void* stream) {
             : launch(linear_tile_kernel<BM, BN, 128, WM, WN, G, STAGES, false>, tiles, 1, 64 * WM * WN * G, a, stream);
 }
 // Which kernel: by the number of tokens, then the largest tile whose grid still covers most of the 256 CUs (us, w one of three in turn, bf16 out):
-//   m <= 32  weights straight into operands      32 x 4096 x 4096: 11.2 against 13.7 on 64 x 64 tiles;  64 x 8192 x 8192: 40.2 against 20.8 - tiles from 33 tokens on
+//   m <= 32  weights straight into operands, wide tiles of channels where they fill the GPU:  32 x 16384 x 4096: 30.9 (NT 1), 20.3 (2), 17.2 (4);  32 x 8192 x 8192: 26.9, 21.9, 25.3
+//                                                32 x 4096 x 4096: 11.2 against 13.7 on 64 x 64 tiles;  64 x 8192 x 8192: 40.2 against 20.8 - tiles from 33 tokens on
 //   256 x 256 from 192 tiles on                  8192^3: 531 against 781 on 128 x 128
 //   64 x 64 at most 256 tiles: four groups       256 x 4096 x 4096: 12.2 against 14.9 with one group;  320 x 4096 x 4096 (320 tiles): 22.9 against 17.0
 int product(const LinearArgs& a, bool al, void* stream) {
-  if (a.m <= 16) return few<float, 1, false>(a, al, stream);
-  if (a.m <= 32) return few<float, 2, false>(a, al, stream);
+  if (a.m <= 16) return al && a.m > kInlineTokens && a.n >= 16384 ? few<float, 4, 1, false>(a, al, stream) : few<float, 1, 1, false>(a, al, stream);
+  if (a.m <= 32) return al && a.n >= 16384 ? few<float, 4, 2, false>(a, al, stream) : al && a.n >= 8192 ? few<float, 2, 2, false>(a, al, stream) : few<float, 1, 2, false>(a, al, stream);
   if (ceil_div(a.m, 256) * ceil_div(a.n, 256) >= 192) return tile<256, 256, 4, 2, 1, 2>(a, al, stream);
   if (ceil_div(a.m, 128) * ceil_div(a.n, 128) >= 192) return tile<128, 128, 2, 2, 1, 2>(a, al, stream);
   if (ceil_div(a.m, 64) * ceil_div(a.n, 64) > 256) return tile<64, 64, 2, 2, 1, 4>(a, al, stream);
@@ -102,9 +105,10 @@ template <class T, class R>
 int norm(const NormArgs& a, bool vector, void* stream) {
   if (!vector || a.cols > 16384) return launch(residual_norm_any_kernel<T, R>, a.rows, 1, 256, a, stream);
   if (a.cols <= 512) return launch(residual_norm_kernel<T, R, 64, 1>, ceil_div(a.rows, 4), 1, 256, a, stream);
+  if (a.cols <= 1024) return launch(residual_norm_kernel<T, R, 64, 2>, ceil_div(a.rows, 4), 1, 256, a, stream);
   if (a.cols <= 2048) return launch(residual_norm_kernel<T, R, 256, 1>, a.rows, 1, 256, a, stream);
   if (a.cols <= 4096) return launch(residual_norm_kernel<T, R, 256, 2>, a.rows, 1, 256, a, stream);
-  if (a.cols <= 8192) return launch(residual_norm_kernel<T, R, 256, 4>, a.rows, 1, 256, a, stream);
+  if (a.cols <= 8192) return launch(residual_norm_kernel<T, R, 512, 2>, a.rows, 1, 512, a, stream);
   return launch(residual_norm_kernel<T, R, 1024, 2>, a.rows, 1, 1024, a, stream);
 }
 
@@ -147,7 +151,11 @@ const char* check_shape(const tha4_diff_attention_args& a) {
 
 template <class T, int D>
 int attention(AttnArgs& a, const Plan& p, void* stream) {
-  if (!p.few) return launch(diff_prompt_kernel<T, D>, (int64_t)a.batch * a.heads * ceil_div(a.q_len, kQueries), 1, 512, a, stream);
+  if (!p.few) {
+    const int64_t heads = (int64_t)a.batch * a.heads;
+    if (heads * ceil_div(a.q_len, 128) >= 256) return launch(diff_prompt_kernel<T, D, 4>, heads * ceil_div(a.q_len, 128), 1, 512, a, stream);
+    return launch(diff_prompt_kernel<T, D, 2>, heads * ceil_div(a.q_len, 64), 1, 256, a, stream);      // (few queries: workgroups of 64 fill more of the 256 CUs)
+  }
   const int64_t tiles = (int64_t)a.batch * a.kv_heads * p.row_tiles;
   const int st = launch(diff_few_kernel<T, D>, tiles * p.splits, 1, 256, a, stream);
   if (st != THA4_OK || p.splits == 1) return st;
@@ -201,7 +209,7 @@ int tha4_linear_i8(const tha4_linear_i8_args* args, void* stream) {
   const bool w16 = g.k % 16 == 0 && aligned(g.w_dev, g.w_row_stride, 1);
   if (!quantised) {
     if (inline_tokens(g))
-      return g.x_dtype == THA4_F32 ? few<float, 1, true>(a, w16, stream) : g.x_dtype == THA4_F16 ? few<f16, 1, true>(a, w16, stream) : few<bf16, 1, true>(a, w16, stream);
+      return g.x_dtype == THA4_F32 ? few<float, 1, 1, true>(a, w16, stream) : g.x_dtype == THA4_F16 ? few<f16, 1, 1, true>(a, w16, stream) : few<bf16, 1, 1, true>(a, w16, stream);
     const int64_t stride = token_stride(g);
     int8_t* q = static_cast<int8_t*>(g.workspace_dev);
     float* scale = reinterpret_cast<float*>(q + g.m * stride);

@@ -69,11 +69,12 @@ THA4_DEV float lambda_of(const AttnArgs& a, int head) {
 }
 
 // ---- prompts: many queries ---------------------------------------------------------------------------------------------------------------
-// A workgroup owns 128 queries of one head: eight waves, wave w the queries 32 (w % 4) .. + 31 of map w / 4 (the maps meet once, at the end: each wave carries one
+// A workgroup owns 32 RG queries of one head: 2 RG waves, wave w the queries 32 (w % RG) .. + 31 of map w / RG (the maps meet once, at the end: each wave carries one
 // map's accumulator, which is what lets 2 x 2d columns fit the registers).  Keys go through LDS in tiles of 64: K of both maps and V.
 // The 16-byte pieces of a K row are permuted so that the 16 lanes the LDS serves together read 16 different slots, those of a V row so that
-// the four rows of a transposing read lie in different quarters of the banks.
-constexpr int kKeys = 64, kQueries = 128;
+// the four rows of a transposing read lie in different quarters of the banks.  Two tiles of LDS: the next one is requested, asynchronously, when everybody has left the one
+// before, and has the time of a whole tile to arrive; one barrier a tile.
+constexpr int kKeys = 64;
 
 template <int D>
 struct Tile {
@@ -83,35 +84,36 @@ struct Tile {
   static THA4_DEV int v_swizzle(int row) { return VP == 8 ? ((row >> 1) & 1) * 4 : (row & 3) * 4; }
 };
 
-// Copies the tile of keys k0 .. k0 + 63 into LDS: per instruction a wave moves 64 pieces, 64 / KP rows of K or 64 / VP rows of V; keys behind the last repeat the last one.
+// Requests the tile of keys k0 .. k0 + 63 into LDS: per copy a wave moves 64 pieces, 64 / KP rows of K or 64 / VP rows of V; keys behind the last repeat the last one.
 // kb, vb: the rows of key k0 (scalar); offsets inside a tile fit 32 bits (the host bounds the strides).
-template <class T, int D>
-THA4_DEV void load_tile(const AttnArgs& a, const T* kb, const T* vb, int left, char* lds) {
+template <class T, int D, int WAVES>
+THA4_DEV void request_tile(const AttnArgs& a, const T* kb, const T* vb, int left, unsigned lds) {
   typedef Tile<D> L;
   const int lane = threadIdx.x & 63, wave = uniform_i32(threadIdx.x >> 6);
-  constexpr int KR = 8 * 64 / L::KP, VR = 8 * 64 / L::VP;              // rows that the eight waves move per instruction
+  constexpr int KR = WAVES * 64 / L::KP, VR = WAVES * 64 / L::VP;      // rows that the waves move together: multiples of 16, after which the swizzles repeat
+  static_assert(KR % 16 == 0 && VR % 4 == 0 && (KR >= kKeys ? KR % kKeys == 0 : kKeys % KR == 0), "every copy of a wave has the same column permutation");
   const unsigned ks = (unsigned)a.ks[1], vs = (unsigned)a.vs[1];
-  const int kw = wave * (KR / 8), krow = kw % kKeys + lane / L::KP;
-  const unsigned kcol = 8 * ((lane % L::KP) ^ L::k_swizzle(krow));     // (the swizzles repeat after 16 rows: the same for every instruction of the wave)
-  const int vrow = wave * (VR / 8) + lane / L::VP;
+  const int kw = wave * (KR / WAVES), krow = kw % kKeys + lane / L::KP;
+  const unsigned kcol = 8 * ((lane % L::KP) ^ L::k_swizzle(krow));
+  const int vrow = wave * (VR / WAVES) + lane / L::VP;
   const unsigned vcol = 8 * ((lane % L::VP) ^ L::v_swizzle(vrow));
 #pragma unroll
-  for (int u = 0; u < L::K_BYTES / 8192; ++u)
-    glds16(kb + (u * KR / kKeys + kw / kKeys) * a.ks[2] + ((unsigned)min(krow + (u * KR) % kKeys, left) * ks + kcol), lds + (u * 8 + wave) * 1024);
+  for (int u = 0; u < L::K_BYTES / 1024 / WAVES; ++u)
+    copy16_async(kb + (u * KR / kKeys + kw / kKeys) * a.ks[2] + ((unsigned)min(krow + (u * KR) % kKeys, left) * ks + kcol), lds + (u * WAVES + wave) * 1024);
 #pragma unroll
-  for (int u = 0; u < L::V_BYTES / 8192; ++u)
-    glds16(vb + ((unsigned)min(vrow + u * VR, left) * vs + vcol), lds + L::K_BYTES + (u * 8 + wave) * 1024);
+  for (int u = 0; u < L::V_BYTES / 1024 / WAVES; ++u)
+    copy16_async(vb + ((unsigned)min(vrow + u * VR, left) * vs + vcol), lds + L::K_BYTES + (u * WAVES + wave) * 1024);
 }
 
 // A tile of which some query sees only a part, with an infinity or a NaN in V: 0 * inf must not reach a query that does not see that key.  The value is added
 // to the accumulators that do see it, and taken out of the tile.  Rare: written for size.
-template <class T, int D>
+template <class T, int D, int THREADS>
 THA4_DEV void quarantine(const AttnArgs& a, char* vt, f32x16 (&acc)[D / 16], int k0, int limit, const uint8_t* mask, int* flag) {
   typedef Tile<D> L;
   const int lane = threadIdx.x & 63;
   auto finite16 = [](unsigned short u) { return sizeof(T) && (std::is_same<T, bf16>::value ? (u & 0x7f80) != 0x7f80 : (u & 0x7c00) != 0x7c00); };
   bool bad = false;
-  for (int p = threadIdx.x; p < L::V_BYTES / 2; p += 512) bad |= !finite16(reinterpret_cast<const unsigned short*>(vt)[p]);
+  for (int p = threadIdx.x; p < L::V_BYTES / 2; p += THREADS) bad |= !finite16(reinterpret_cast<const unsigned short*>(vt)[p]);
   if (bad) *flag = 1;
   __syncthreads();
   const bool any = *flag != 0;
@@ -134,7 +136,7 @@ THA4_DEV void quarantine(const AttnArgs& a, char* vt, f32x16 (&acc)[D / 16], int
     }
   }
   __syncthreads();
-  for (int p = threadIdx.x; p < L::V_BYTES / 2; p += 512) {
+  for (int p = threadIdx.x; p < L::V_BYTES / 2; p += THREADS) {
     unsigned short* u = reinterpret_cast<unsigned short*>(vt) + p;
     if (!finite16(*u)) *u = 0;
   }
@@ -142,24 +144,25 @@ THA4_DEV void quarantine(const AttnArgs& a, char* vt, f32x16 (&acc)[D / 16], int
   __syncthreads();
 }
 
-template <class T, int D>
-__global__ void __launch_bounds__(512, 2) diff_prompt_kernel(AttnArgs a) {
+template <class T, int D, int RG>
+__global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
   warm_kernarg<(int)sizeof(AttnArgs)>();
   typedef Tile<D> L;
   typedef typename Mat<T>::v8 v8;
   constexpr int VT = D / 16;                                           // tiles of 32 value columns
   constexpr int J = D == 128 ? 1 : 2;                                  // groups of 32 keys a softmax step takes: one where the accumulator leaves no registers for two
-  constexpr int JOIN = 4 * VT * 16 * 64 * 4;                           // bytes in which the second maps' results meet the first's
-  __shared__ __attribute__((aligned(16))) char lds[L::BYTES > JOIN ? L::BYTES : JOIN];
+  constexpr int JOIN = RG * VT * 16 * 64 * 4;                          // bytes in which the second maps' results meet the first's
+  constexpr int kQueries = 32 * RG;
+  __shared__ __attribute__((aligned(16))) char lds[2 * L::BYTES > JOIN ? 2 * L::BYTES : JOIN];
   __shared__ int flag;
-  const int lane = threadIdx.x & 63, wave = uniform_i32(threadIdx.x >> 6), map = wave >> 2, h = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = uniform_i32(threadIdx.x >> 6), map = wave / RG, h = lane >> 5;
   const int bh = blockIdx.x % (a.batch * a.heads), b = bh / a.heads, head = bh % a.heads;
   const int q0 = ((int)(gridDim.x / (a.batch * a.heads)) - 1 - (int)(blockIdx.x / (a.batch * a.heads))) * kQueries;     // the longest rows of a causal map first
   const Lengths n = lengths_of(a, b);
   if (q0 >= n.q) return;
   if (threadIdx.x == 0) flag = 0;
   const int kv = head / a.group, off = n.k - n.q;
-  const int qw = q0 + 32 * (wave & 3), qi = qw + (lane & 31), row = min(qi, n.q - 1);
+  const int qw = q0 + 32 * (wave % RG), qi = qw + (lane & 31), row = min(qi, n.q - 1);
   const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + row * a.qs[1] + (2 * head + map) * a.qs[2];
   const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + 2 * kv * a.ks[2];
   const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2];
@@ -175,14 +178,19 @@ __global__ void __launch_bounds__(512, 2) diff_prompt_kernel(AttnArgs a) {
   for (int t = 0; t < VT; ++t) acc[t] = f32x16{0};
   float m = -INFINITY, l = 0.0f;
 
+  const unsigned lds_at = lds_address(lds);
+  auto request = [&](int k0) {
+    request_tile<T, D, 2 * RG>(a, k + (int64_t)k0 * a.ks[1], v + (int64_t)k0 * a.vs[1], n.k - 1 - k0, lds_at + (k0 / kKeys % 2) * L::BYTES);
+  };
+  if (wg_end > 0) request(0);
   auto tile = [&](int k0, auto part_) {
     constexpr bool part = decltype(part_)::value;
-    __syncthreads();
-    load_tile<T, D>(a, k + (int64_t)k0 * a.ks[1], v + (int64_t)k0 * a.vs[1], n.k - 1 - k0, lds);
-    __syncthreads();
-    const char* kt = lds + map * (L::K_BYTES / 2);
-    char* vt = lds + L::K_BYTES;
-    if constexpr (part) quarantine<T, D>(a, vt, acc, k0, limit, mask, &flag);
+    THA4_BARRIER_KEEP(0);                                              // this tile is there, and everybody has left the other one
+    if (k0 + kKeys < wg_end) request(k0 + kKeys);
+    char* const tile_at = lds + (k0 / kKeys % 2) * L::BYTES;
+    const char* kt = tile_at + map * (L::K_BYTES / 2);
+    char* vt = tile_at + L::K_BYTES;
+    if constexpr (part) quarantine<T, D, 128 * RG>(a, vt, acc, k0, limit, mask, &flag);
 #pragma unroll
     for (int j0 = 0; j0 < 2; j0 += J) {
       f32x16 s[J];
@@ -253,7 +261,7 @@ __global__ void __launch_bounds__(512, 2) diff_prompt_kernel(AttnArgs a) {
   for (; k0 < wg_end; k0 += kKeys) tile(k0, std::true_type());
 
   l += other_half(l);
-  float* meet = reinterpret_cast<float*>(lds) + (wave & 3) * (VT * 16 * 64) + lane;
+  float* meet = reinterpret_cast<float*>(lds) + (wave % RG) * (VT * 16 * 64) + lane;
   __syncthreads();
   if (map == 1) {
     const float lam = lambda_of<D>(a, head), w = l > 0.0f || l != l ? lam / l : 0.0f;      // (no key seen: nothing)

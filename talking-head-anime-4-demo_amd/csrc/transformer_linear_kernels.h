@@ -142,23 +142,26 @@ THA4_DEV i32x4 piece16(const int8_t* p, int64_t k, int64_t n) {
   return v;
 }
 
-// Few tokens: the weights are the traffic.  A workgroup owns 16 channels x 16 MT tokens; its 8 waves take turns of 128 k, weights straight from memory into
-// matrix-instruction operands (nothing else would reuse them), AHEAD turns of them on their way at any time, and their exact partial sums meet in LDS.
+// Few tokens: the weights are the traffic.  A workgroup owns 16 NT channels x 16 MT tokens; its 8 waves take turns of 128 k, weights straight from memory into
+// matrix-instruction operands (nothing else would reuse them), AHEAD turns of them on their way at any time, and their exact partial sums meet in LDS.  Every workgroup reads all the tokens, through L2: with 16 of them and one tile of channels that is as much again as the weights.
+// NT tiles for each token operand where there are channels enough to fill the GPU (16 x 16384 x 8192: NT 1 38.9 us, 2 35.6, 4 32.7 = 4.1 TB/s; one token: NT 1 28.1 us = 4.8 TB/s, 4 30.6).
 // INLINE: x is float (XT) and at most kInlineTokens x kInlineK: every workgroup quantises the tokens itself, into LDS, while its first weights are on their
 // way - a few hundred instructions against a launch of their own.
 constexpr int kInlineTokens = 4, kInlineBytes = 32768;
 
-template <class XT, int MT, bool ALIGNED, bool INLINE>
+template <class XT, int NT, int MT, bool ALIGNED, bool INLINE>
 __global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
   warm_kernarg<(int)sizeof(LinearArgs)>();
-  constexpr int WAVES = 8, AHEAD = MT == 1 ? 4 : 2;
-  __shared__ i32x4 part[WAVES][MT][64];
+  constexpr int WAVES = 8, AHEAD = NT * MT >= 4 ? 1 : NT * MT == 2 ? 2 : 4;
+  __shared__ i32x4 part[WAVES][NT * MT][64];
   __shared__ __attribute__((aligned(16))) int8_t xq[INLINE ? kInlineBytes : 16];
   __shared__ float xscale[INLINE ? kInlineTokens : 1], slot[WAVES];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 15, g = lane >> 4;
-  const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * (16 * MT);
-  const int8_t* w = a.w + (n0 + r < a.n ? n0 + r : a.n - 1) * a.w_stride;   // (a channel behind the last: the last again, not stored)
+  const int64_t n0 = (int64_t)blockIdx.x * (16 * NT), m0 = (int64_t)blockIdx.y * (16 * MT);
+  const int8_t* w[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) w[i] = a.w + (n0 + 16 * i + r < a.n ? n0 + 16 * i + r : a.n - 1) * a.w_stride;   // (a channel behind the last: the last again, not stored)
   const int8_t* x[MT];
   int64_t xk[MT];
 #pragma unroll
@@ -167,13 +170,15 @@ __global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
     xk[i] = row < a.m ? a.k : 0;                                            // a token behind the last: zeros, nothing is read
     x[i] = INLINE ? xq + (row < a.m ? row : 0) * a.k : static_cast<const int8_t*>(a.x) + (row < a.m ? row : 0) * a.x_stride;
   }
-  i32x4 acc[MT];
+  i32x4 acc[NT][MT];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) acc[i] = i32x4{0, 0, 0, 0};
-  i32x4 wf[AHEAD][2], xf[AHEAD][2][MT];
+  for (int i = 0; i < NT * MT; ++i) acc[i / MT][i % MT] = i32x4{0, 0, 0, 0};
+  i32x4 wf[AHEAD][2][NT], xf[AHEAD][2][MT];
   auto weights = [&](int t, int64_t k0) {                                   // (behind the row's end: zeros, nothing is read)
 #pragma unroll
-    for (int s = 0; s < 2; ++s) wf[t][s] = piece16<ALIGNED>(w, k0 + 64 * s + 16 * g, a.k);
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) wf[t][s][i] = piece16<ALIGNED>(w[i], k0 + 64 * s + 16 * g, a.k);
   };
   auto tokens = [&](int t, int64_t k0) {
 #pragma unroll
@@ -218,25 +223,25 @@ __global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[t][s], xf[t][s][i], acc[i], 0, 0, 0);
+        for (int i = 0; i < NT * MT; ++i) acc[i / MT][i % MT] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[t][s][i / MT], xf[t][s][i % MT], acc[i / MT][i % MT], 0, 0, 0);
       weights(t, next);
       if constexpr (!INLINE) tokens(t, next);
     }
   }
 #pragma unroll
-  for (int i = 0; i < MT; ++i) part[wave][i][lane] = acc[i];
+  for (int i = 0; i < NT * MT; ++i) part[wave][i][lane] = acc[i / MT][i % MT];
   __syncthreads();
-  for (int u = threadIdx.x; u < MT * 64; u += 512) {
+  for (int u = threadIdx.x; u < NT * MT * 64; u += 512) {
     const int i = u >> 6, l = u & 63;
     i32x4 s = part[0][i][l];
 #pragma unroll
     for (int v = 1; v < WAVES; ++v) s += part[v][i][l];
-    const int64_t row = m0 + 16 * i + (l & 15);
+    const int64_t row = m0 + 16 * (i % MT) + (l & 15);
     if (row >= a.m) continue;
     const float xs = INLINE ? xscale[row] : a.xs[row];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int64_t col = n0 + 4 * (l >> 4) + e;
+      const int64_t col = n0 + 16 * (i / MT) + 4 * (l >> 4) + e;
       if (col >= a.n) continue;
       float v = (float)s[e] * xs * a.ws[col];
       if (a.bias) v += a.bias[col];

@@ -39,7 +39,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) residual_norm_kernel(No
 
   float h[NV][8];
   Raw8<R> res[NV];
-  float gate[NV][8];
+  Raw8<T> gate[NV];                                      // (of the gate's own type only if that is T; an fp32 gate beside 16-bit rows is read where it is used)
   bool in[NV];
   int c[NV];
 #pragma unroll
@@ -54,9 +54,10 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) residual_norm_kernel(No
     for (int j = 0; j < NV; ++j) raw[j] = fetch8(branch + c[j]);
 #pragma unroll
     for (int j = 0; j < NV; ++j) res[j] = fetch8(residual + c[j]);
-    if (a.gate) {
+    const bool gate_here = a.gate && (std::is_same<T, float>::value || !a.gate_f32);
+    if (gate_here) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) param8<T>(a.gate, gate_at + c[j], a.gate_f32 != 0, gate[j]);
+      for (int j = 0; j < NV; ++j) gate[j] = fetch8(static_cast<const T*>(a.gate) + gate_at + c[j]);
     }
     float sum = 0.0f;
 #pragma unroll
@@ -87,16 +88,18 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) residual_norm_kernel(No
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      float w[8], b[8], r[8];
+      float w[8], b[8], r[8], g[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) { w[e] = 1.0f; b[e] = 0.0f; }
       if (a.post_w) param8<T>(a.post_w, c[j], pf, w);
       if (a.post_b) param8<T>(a.post_b, c[j], pf, b);
       unpack8(res[j], r);
+      if (gate_here) unpack8(gate[j], g);
+      else if (a.gate) unpack8(fetch8(static_cast<const float*>(a.gate) + gate_at + c[j]), g);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float v = fmaf(h[j][e] * k, w[e], b[e]);
-        if (a.gate) v *= a.sigmoid ? sigmoid(gate[j][e]) : gate[j][e];
+        if (a.gate) v *= a.sigmoid ? sigmoid(g[e]) : g[e];
         h[j][e] = v;
         r[e] *= a.residual_scale;
       }
