@@ -24,7 +24,7 @@ struct AttnArgs {
   int64_t lambda_vs, lambda_hs;
   int32_t batch, q_len, k_len, heads, kv_heads, group, causal, norm;
   int32_t row_tiles, splits, chunk, part_rows;
-  float c, lambda_init, eps;                   // c = scale * log2(e): the softmax is taken in powers of two
+  float c, slack, lambda_init, eps;            // c = scale * log2(e): the softmax is taken in powers of two; slack = 8 / c
 };
 
 template <class T> struct Mat;
@@ -47,7 +47,13 @@ template <class V8>
 THA4_DEV V8 join(s16x4 a, s16x4 b) { return __builtin_bit_cast(V8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)); }
 
 THA4_DEV float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
-THA4_DEV float other_half(float v) { return __shfl_xor(v, 32, 64); }
+// f of the values that lanes i and i + 32 hold, in both: v_permlane32_swap of v with itself leaves the lower half's values in one result, the upper half's in the other
+template <class F>
+THA4_DEV float both_halves(float v, F f) {
+  const unsigned u = __float_as_uint(v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 
 struct Lengths { int q, k; };
 THA4_DEV Lengths lengths_of(const AttnArgs& a, int b) {
@@ -162,7 +168,7 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
   if (q0 >= n.q) return;
   if (threadIdx.x == 0) flag = 0;
   const int kv = head / a.group, off = n.k - n.q;
-  const int qw = q0 + 32 * (wave % RG), qi = qw + (lane & 31), row = min(qi, n.q - 1);
+  const int qw = q0 + 32 * (wave % RG), row = min(qw + (lane & 31), n.q - 1);
   const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + row * a.qs[1] + (2 * head + map) * a.qs[2];
   const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + 2 * kv * a.ks[2];
   const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2];
@@ -191,19 +197,40 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
     const char* kt = tile_at + map * (L::K_BYTES / 2);
     char* vt = tile_at + L::K_BYTES;
     if constexpr (part) quarantine<T, D, 128 * RG>(a, vt, acc, k0, limit, mask, &flag);
+    // Operands leave LDS ahead of their products: V's first ones in front of the softmax, each later one behind the product with its predecessor (its registers), the
+    // next K under the products with V
+    int ln = lane;
+    if constexpr (part) asm volatile("" : "+v"(ln));                   // (the few partial tiles compute their addresses again: kept for the whole loop, they would cost it registers)
+    const int lh = ln >> 5;
+    auto v_operand = [&](int u, int t) {                               // k slot (h, e) of step u holds key 16 u + 8 (e / 4) + 4 h + e % 4: the accumulator layout of S^T
+      const int r0 = 16 * u + 4 * lh + ((ln & 15) >> 2), piece = 4 * t + 2 * ((ln >> 4) & 1) + ((ln & 3) >> 1), in = 8 * (ln & 1);
+      const s16x4 lo = read_transposed(vt + (r0 * L::VP + (piece ^ L::v_swizzle(r0))) * 16 + in);
+      const s16x4 hi = read_transposed(vt + ((r0 + 8) * L::VP + (piece ^ L::v_swizzle(r0 + 8))) * 16 + in);
+      return join<v8>(lo, hi);
+    };
+    auto k_operand = [&](int i, int u) {
+      const int r = 32 * i + (ln & 31);
+      return *reinterpret_cast<const v8*>(kt + (r * L::KP + ((2 * u + lh) ^ L::k_swizzle(r))) * 16);
+    };
+    constexpr int AHEAD = VT < 4 ? VT : 4, KS = D / 16;                // products whose operands are on their way; products of a group of keys
+    v8 kf[AHEAD], vf[AHEAD];
+#pragma unroll
+    for (int p = 0; p < AHEAD; ++p) kf[p] = k_operand(p / KS, p % KS);
 #pragma unroll
     for (int j0 = 0; j0 < 2; j0 += J) {
       f32x16 s[J];
 #pragma unroll
-      for (int i = 0; i < J; ++i) {
-        s[i] = f32x16{0};
-        const int r = 32 * (j0 + i) + (lane & 31);
+      for (int i = 0; i < J; ++i) s[i] = f32x16{0};
 #pragma unroll
-        for (int u = 0; u < D / 16; ++u) {
-          const v8 kf = *reinterpret_cast<const v8*>(kt + (r * L::KP + ((2 * u + h) ^ L::k_swizzle(r))) * 16);
-          s[i] = Mat<T>::mma32(kf, qf[u], s[i]);
-        }
+      for (int p = 0; p < J * KS; ++p) {
+        s[p / KS] = Mat<T>::mma32(kf[p % AHEAD], qf[p % KS], s[p / KS]);
+        if (p + AHEAD < J * KS) kf[p % AHEAD] = k_operand(j0 + (p + AHEAD) / KS, (p + AHEAD) % KS);
+        if (p % AHEAD == AHEAD - 1) THA4_SCHED_FENCE();
       }
+      THA4_SCHED_FENCE();
+#pragma unroll
+      for (int t = 0; t < AHEAD; ++t) vf[t] = v_operand(2 * j0, t);
+      THA4_SCHED_FENCE();
       if constexpr (part) {
 #pragma unroll
         for (int i = 0; i < J; ++i)
@@ -218,15 +245,17 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
             s[i][r] = seen ? s[i][r] : -INFINITY;
           }
       }
-      THA4_SCHED_FENCE();
       float top = s[0][0];
 #pragma unroll
       for (int i = 0; i < J; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
-      top = fmaxf(top, other_half(top));
-      if (__any(top > m)) {
-        const float now = fmaxf(m, top), w = now == -INFINITY ? 1.0f : exp2_((m - now) * a.c);
+      top = both_halves(top, Max());
+      // The reference point of the exponents follows the maximum only when that has outgrown it by 2^8 (in the first tiles of nearly every row, seldom later): weights stay below 2^8, which
+      // fp16 and bf16 hold with their full precision, and the accumulator is left alone in most steps
+      const float now = top > m + a.slack ? top : m;
+      if (__any(now != m)) {
+        const float w = now == -INFINITY ? 1.0f : exp2_((m - now) * a.c);
         l *= w;
 #pragma unroll
         for (int t = 0; t < VT; ++t) acc[t] *= w;
@@ -243,24 +272,24 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
           pf[2 * i + r / 8][r % 8] = (T)p;
         }
       THA4_SCHED_FENCE();
-      // k slot (h, e) of the product's step u holds key 16 u + 8 (e / 4) + 4 h + e % 4: the accumulator layout of S^T
 #pragma unroll
-      for (int u = 0; u < 2 * J; ++u)
+      for (int p = 0; p < 2 * J * VT; ++p) {
+        acc[p % VT] = Mat<T>::mma32(vf[p % AHEAD], pf[p / VT], acc[p % VT]);
+        const int next = p + AHEAD;
+        if (next < 2 * J * VT) vf[p % AHEAD] = v_operand(2 * j0 + next / VT, next % VT);
+        if (p % AHEAD == AHEAD - 1) THA4_SCHED_FENCE();
+      }
+      if (j0 + J < 2) {
 #pragma unroll
-        for (int t = 0; t < VT; ++t) {
-          const int r0 = 32 * j0 + 16 * u + 4 * h + ((lane & 15) >> 2), piece = 4 * t + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), in = 8 * (lane & 1);
-          const s16x4 lo = read_transposed(vt + (r0 * L::VP + (piece ^ L::v_swizzle(r0))) * 16 + in);
-          const s16x4 hi = read_transposed(vt + ((r0 + 8) * L::VP + (piece ^ L::v_swizzle(r0 + 8))) * 16 + in);
-          acc[t] = Mat<T>::mma32(join<v8>(lo, hi), pf[u], acc[t]);
-        }
-      THA4_SCHED_FENCE();
+        for (int p = 0; p < AHEAD; ++p) kf[p] = k_operand(j0 + J, p);
+      }
     }
   };
   int k0 = 0;
   for (; k0 + kKeys <= wg_full; k0 += kKeys) tile(k0, std::false_type());
   for (; k0 < wg_end; k0 += kKeys) tile(k0, std::true_type());
 
-  l += other_half(l);
+  l = both_halves(l, Add());
   float* meet = reinterpret_cast<float*>(lds) + (wave % RG) * (VT * 16 * 64) + lane;
   __syncthreads();
   if (map == 1) {
@@ -281,7 +310,10 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
       acc[t][r] = fmaf(acc[t][r], w, -meet[(t * 16 + r) * 64]);
       ss = fmaf(acc[t][r], acc[t][r], ss);
     }
-  ss += other_half(ss);
+  ss = both_halves(ss, Add());
+  int le = threadIdx.x & 63;
+  asm volatile("" : "+v"(le));                                        // (the query's number again: not worth a register throughout the loop)
+  const int qi = qw + (le & 31);
   if (qi >= n.q) return;
   const float g = a.norm ? (1.0f - a.lambda_init) / sqrtf(ss * (1.0f / (2 * D)) + a.eps) : 1.0f;
   T* out = static_cast<T*>(a.out) + b * a.os[0] + qi * a.os[1] + head * a.os[2];
@@ -616,7 +648,7 @@ __global__ void __launch_bounds__(512) diff_join_kernel(AttnArgs a) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     for (int s = lane; s < used; s += 64) M[i] = fmaxf(M[i], stat[2 * i][s]);
-    M[i] = wave_reduce(M[i], MaxAbs());
+    M[i] = wave_reduce(M[i], Max());
     for (int s = lane; s < used; s += 64) S[i] += stat[2 * i][s] == -INFINITY ? stat[2 * i + 1][s] : stat[2 * i + 1][s] * exp2_((stat[2 * i][s] - M[i]) * a.c);
     S[i] = wave_reduce(S[i], Add());
   }

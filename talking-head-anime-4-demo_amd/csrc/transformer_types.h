@@ -71,7 +71,7 @@ THA4_DEV float param1(const void* p, int64_t at, bool is_f32) {
 }
 
 struct Add { THA4_DEV float operator()(float a, float b) const { return a + b; } };
-struct MaxAbs { THA4_DEV float operator()(float a, float b) const { return fmaxf(a, b); } };
+struct Max { THA4_DEV float operator()(float a, float b) const { return fmaxf(a, b); } };
 
 template <class F>
 THA4_DEV float wave_reduce(float v, F f) {                       // a butterfly: every lane ends with the same bits
