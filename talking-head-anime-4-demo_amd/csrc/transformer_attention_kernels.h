@@ -55,6 +55,29 @@ THA4_DEV float both_halves(float v, F f) {
   return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// whether one of the 16-bit numbers in a 16-byte piece is an infinity or a NaN (all ones in the exponent: one more there carries into the sign's place)
+template <class T>
+THA4_DEV bool not_finite(const u32x4& p) {
+  constexpr unsigned M = std::is_same<T, bf16>::value ? 0x7f807f80u : 0x7c007c00u, one = std::is_same<T, bf16>::value ? 0x00800080u : 0x04000400u;
+  unsigned r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r |= (p[i] & M) + one;
+  return (r & 0x80008000u) != 0;
+}
+template <class T>
+THA4_DEV bool not_finite(T v) { return (__builtin_bit_cast(unsigned short, v) & (std::is_same<T, bf16>::value ? 0x7f80 : 0x7c00)) == (std::is_same<T, bf16>::value ? 0x7f80 : 0x7c00); }
+// zeros in their places, in the pieces `first`, `first + step`, ... of `bytes` bytes of LDS
+template <class T>
+THA4_DEV void clear_not_finite(char* lds, int bytes, int first, int step) {
+  for (int p = first; p < bytes / 16; p += step) {
+    u32x4 v = reinterpret_cast<u32x4*>(lds)[p];
+    if (!not_finite<T>(v)) continue;
+    T* e = reinterpret_cast<T*>(lds) + 8 * p;
+    for (int i = 0; i < 8; ++i)
+      if (not_finite(e[i])) e[i] = (T)0.0f;
+  }
+}
+
 struct Lengths { int q, k; };
 THA4_DEV Lengths lengths_of(const AttnArgs& a, int b) {
   Lengths n;
@@ -76,56 +99,61 @@ THA4_DEV float lambda_of(const AttnArgs& a, int head) {
 
 // ---- prompts: many queries ---------------------------------------------------------------------------------------------------------------
 // A workgroup owns 32 RG queries of one head: 2 RG waves, wave w the queries 32 (w % RG) .. + 31 of map w / RG (the maps meet once, at the end: each wave carries one
-// map's accumulator, which is what lets 2 x 2d columns fit the registers).  Keys go through LDS in tiles of 64: K of both maps and V.
+// map's accumulator, which is what lets 2 x 2d columns fit the registers).  Keys go through LDS in groups, K of both maps and V, through a ring of four groups:
+// copies are asynchronous and have two to three groups' time to arrive.
 // The 16-byte pieces of a K row are permuted so that the 16 lanes the LDS serves together read 16 different slots, those of a V row so that
-// the four rows of a transposing read lie in different quarters of the banks.  Two tiles of LDS: the next one is requested, asynchronously, when everybody has left the one
-// before, and has the time of a whole tile to arrive; one barrier a tile.
-constexpr int kKeys = 64;
-
+// the four rows of a transposing read lie in different quarters of the banks (no conflicts by the counters).
+//
+// Two waves share a SIMD: one of each map.  A group costs a wave a stretch of matrix products (with V of the group before, then with K of this one) and a stretch of
+// vector arithmetic (the softmax); the two waves run them in opposite phases, a barrier between the phases, so that one's arithmetic runs under the other's products.
 template <int D>
 struct Tile {
+  static constexpr int J = D == 128 ? 1 : 2, KEYS = 32 * J, SLOTS = 4;  // 32-key tiles of a group: one where the accumulator leaves no registers for two
   static constexpr int KP = D / 8, VP = D / 4;                         // 16-byte pieces of a K row (one map), of a V row
-  static constexpr int K_BYTES = 2 * kKeys * KP * 16, V_BYTES = kKeys * VP * 16, BYTES = K_BYTES + V_BYTES;
+  static constexpr int K_BYTES = 2 * KEYS * KP * 16, V_BYTES = KEYS * VP * 16, BYTES = K_BYTES + V_BYTES;
   static THA4_DEV int k_swizzle(int row) { return (row / (16 / KP)) & (KP - 1); }
   static THA4_DEV int v_swizzle(int row) { return VP == 8 ? ((row >> 1) & 1) * 4 : (row & 3) * 4; }
 };
 
-// Requests the tile of keys k0 .. k0 + 63 into LDS: per copy a wave moves 64 pieces, 64 / KP rows of K or 64 / VP rows of V; keys behind the last repeat the last one.
-// kb, vb: the rows of key k0 (scalar); offsets inside a tile fit 32 bits (the host bounds the strides).
+// Request K (of both maps) or V of a group into LDS: per copy a wave moves 64 pieces, 64 / KP rows of K or 64 / VP rows of V; keys behind row `left` repeat it.
+// kb, vb: the group's first rows (scalar); offsets inside a group fit 32 bits (the host bounds the strides).
 template <class T, int D, int WAVES>
-THA4_DEV void request_tile(const AttnArgs& a, const T* kb, const T* vb, int left, unsigned lds) {
+THA4_DEV void request_group_k(const AttnArgs& a, const T* kb, int left, unsigned lds) {
   typedef Tile<D> L;
   const int lane = threadIdx.x & 63, wave = uniform_i32(threadIdx.x >> 6);
-  constexpr int KR = WAVES * 64 / L::KP, VR = WAVES * 64 / L::VP;      // rows that the waves move together: multiples of 16, after which the swizzles repeat
-  static_assert(KR % 16 == 0 && VR % 4 == 0 && (KR >= kKeys ? KR % kKeys == 0 : kKeys % KR == 0), "every copy of a wave has the same column permutation");
-  const unsigned ks = (unsigned)a.ks[1], vs = (unsigned)a.vs[1];
-  const int kw = wave * (KR / WAVES), krow = kw % kKeys + lane / L::KP;
-  const unsigned kcol = 8 * ((lane % L::KP) ^ L::k_swizzle(krow));
-  const int vrow = wave * (VR / WAVES) + lane / L::VP;
-  const unsigned vcol = 8 * ((lane % L::VP) ^ L::v_swizzle(vrow));
+  constexpr int KR = WAVES * 64 / L::KP;                               // rows that the waves move together: a multiple of 16, after which the swizzle repeats
+  static_assert(KR % 16 == 0 && (KR >= L::KEYS ? KR % L::KEYS == 0 : L::KEYS % KR == 0), "every copy of a wave has the same column permutation and one map");
+  const int kw = wave * (KR / WAVES), row = kw % L::KEYS + lane / L::KP;
+  const unsigned col = 8 * ((lane % L::KP) ^ L::k_swizzle(row));
 #pragma unroll
   for (int u = 0; u < L::K_BYTES / 1024 / WAVES; ++u)
-    copy16_async(kb + (u * KR / kKeys + kw / kKeys) * a.ks[2] + ((unsigned)min(krow + (u * KR) % kKeys, left) * ks + kcol), lds + (u * WAVES + wave) * 1024);
+    copy16_async(kb + (u * KR / L::KEYS + kw / L::KEYS) * a.ks[2] + ((unsigned)min(row + (u * KR) % L::KEYS, left) * (unsigned)a.ks[1] + col), lds + (u * WAVES + wave) * 1024);
+}
+template <class T, int D, int WAVES>
+THA4_DEV void request_group_v(const AttnArgs& a, const T* vb, int left, unsigned lds) {
+  typedef Tile<D> L;
+  const int lane = threadIdx.x & 63, wave = uniform_i32(threadIdx.x >> 6);
+  constexpr int VR = WAVES * 64 / L::VP;
+  static_assert(VR % 4 == 0, "every copy of a wave has the same column permutation");
+  const int row = wave * (VR / WAVES) + lane / L::VP;
+  const unsigned col = 8 * ((lane % L::VP) ^ L::v_swizzle(row));
 #pragma unroll
   for (int u = 0; u < L::V_BYTES / 1024 / WAVES; ++u)
-    copy16_async(vb + ((unsigned)min(vrow + u * VR, left) * vs + vcol), lds + L::K_BYTES + (u * WAVES + wave) * 1024);
+    copy16_async(vb + ((unsigned)min(row + u * VR, left) * (unsigned)a.vs[1] + col), lds + L::K_BYTES + (u * WAVES + wave) * 1024);
 }
 
-// A tile of which some query sees only a part, with an infinity or a NaN in V: 0 * inf must not reach a query that does not see that key.  The value is added
-// to the accumulators that do see it, and taken out of the tile.  Rare: written for size.
+// A group of which some query sees only a part, with an infinity or a NaN in V: 0 * inf must not reach a query that does not see that key.  The value is added
+// to the accumulators that do see it, and taken out of the group.  Rare: written for size.
 template <class T, int D, int THREADS>
 THA4_DEV void quarantine(const AttnArgs& a, char* vt, f32x16 (&acc)[D / 16], int k0, int limit, const uint8_t* mask, int* flag) {
   typedef Tile<D> L;
   const int lane = threadIdx.x & 63;
-  auto finite16 = [](unsigned short u) { return sizeof(T) && (std::is_same<T, bf16>::value ? (u & 0x7f80) != 0x7f80 : (u & 0x7c00) != 0x7c00); };
   bool bad = false;
-  for (int p = threadIdx.x; p < L::V_BYTES / 2; p += THREADS) bad |= !finite16(reinterpret_cast<const unsigned short*>(vt)[p]);
+  for (int p = threadIdx.x; p < L::V_BYTES / 16; p += THREADS) bad |= not_finite<T>(reinterpret_cast<const u32x4*>(vt)[p]);
   if (bad) *flag = 1;
   __syncthreads();
-  const bool any = *flag != 0;
-  __syncthreads();
-  if (!any) return;
-  for (int key = 0; key < kKeys; ++key) {
+  if (*flag == 0) return;                                              // (set again behind another barrier at the earliest)
+  for (int key = 0; key < L::KEYS; ++key) {
     const bool seen = k0 + key < limit && (!mask || mask[(int64_t)(k0 + key) * a.ms[3]]);
     const T* row = reinterpret_cast<const T*>(vt + key * L::VP * 16);
     int h = lane >> 5;
@@ -136,16 +164,13 @@ THA4_DEV void quarantine(const AttnArgs& a, char* vt, f32x16 (&acc)[D / 16], int
       for (int r = 0; r < 16; ++r) {
         const int dv = 32 * t + 8 * (r / 4) + 4 * h + r % 4;
         const T val = row[8 * ((dv / 8) ^ L::v_swizzle(key)) + dv % 8];
-        if (seen && !finite16(__builtin_bit_cast(unsigned short, val))) acc[t][r] += (float)val;
+        if (seen && not_finite(val)) acc[t][r] += (float)val;
       }
       THA4_SCHED_FENCE();                                              // (a few values at a time: nothing here may cost the main loop registers)
     }
   }
   __syncthreads();
-  for (int p = threadIdx.x; p < L::V_BYTES / 2; p += THREADS) {
-    unsigned short* u = reinterpret_cast<unsigned short*>(vt) + p;
-    if (!finite16(*u)) *u = 0;
-  }
+  clear_not_finite<T>(vt, L::V_BYTES, threadIdx.x, THREADS);
   if (threadIdx.x == 0) *flag = 0;
   __syncthreads();
 }
@@ -156,10 +181,11 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
   typedef Tile<D> L;
   typedef typename Mat<T>::v8 v8;
   constexpr int VT = D / 16;                                           // tiles of 32 value columns
-  constexpr int J = D == 128 ? 1 : 2;                                  // groups of 32 keys a softmax step takes: one where the accumulator leaves no registers for two
+  constexpr int J = L::J, KS = D / 16, AHEAD = D == 32 ? 4 : 8;        // products of 32 keys with K; operands on their way from LDS
   constexpr int JOIN = RG * VT * 16 * 64 * 4;                          // bytes in which the second maps' results meet the first's
+  constexpr int BATCH = L::BYTES / 1024 / (2 * RG);                    // copies of a wave and group
   constexpr int kQueries = 32 * RG;
-  __shared__ __attribute__((aligned(16))) char lds[2 * L::BYTES > JOIN ? 2 * L::BYTES : JOIN];
+  __shared__ __attribute__((aligned(16))) char lds[L::SLOTS * L::BYTES > JOIN ? L::SLOTS * L::BYTES : JOIN];
   __shared__ int flag;
   const int lane = threadIdx.x & 63, wave = uniform_i32(threadIdx.x >> 6), map = wave / RG, h = lane >> 5;
   const int bh = blockIdx.x % (a.batch * a.heads), b = bh / a.heads, head = bh % a.heads;
@@ -185,109 +211,133 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
   float m = -INFINITY, l = 0.0f;
 
   const unsigned lds_at = lds_address(lds);
-  auto request = [&](int k0) {
-    request_tile<T, D, 2 * RG>(a, k + (int64_t)k0 * a.ks[1], v + (int64_t)k0 * a.vs[1], n.k - 1 - k0, lds_at + (k0 / kKeys % 2) * L::BYTES);
+  const int groups = (max(wg_end, 0) + L::KEYS - 1) / L::KEYS, whole = max(wg_full, 0) / L::KEYS;      // the first `whole` groups are seen wholly by everybody
+  auto request_k = [&](int g) {
+    if (g < groups) request_group_k<T, D, 2 * RG>(a, k + (int64_t)g * L::KEYS * a.ks[1], n.k - 1 - g * L::KEYS, lds_at + g % L::SLOTS * L::BYTES);
   };
-  if (wg_end > 0) request(0);
-  auto tile = [&](int k0, auto part_) {
-    constexpr bool part = decltype(part_)::value;
-    THA4_BARRIER_KEEP(0);                                              // this tile is there, and everybody has left the other one
-    if (k0 + kKeys < wg_end) request(k0 + kKeys);
-    char* const tile_at = lds + (k0 / kKeys % 2) * L::BYTES;
-    const char* kt = tile_at + map * (L::K_BYTES / 2);
-    char* vt = tile_at + L::K_BYTES;
-    if constexpr (part) quarantine<T, D, 128 * RG>(a, vt, acc, k0, limit, mask, &flag);
-    // Operands leave LDS ahead of their products: V's first ones in front of the softmax, each later one behind the product with its predecessor (its registers), the
-    // next K under the products with V
-    int ln = lane;
-    if constexpr (part) asm volatile("" : "+v"(ln));                   // (the few partial tiles compute their addresses again: kept for the whole loop, they would cost it registers)
-    const int lh = ln >> 5;
-    auto v_operand = [&](int u, int t) {                               // k slot (h, e) of step u holds key 16 u + 8 (e / 4) + 4 h + e % 4: the accumulator layout of S^T
-      const int r0 = 16 * u + 4 * lh + ((ln & 15) >> 2), piece = 4 * t + 2 * ((ln >> 4) & 1) + ((ln & 3) >> 1), in = 8 * (ln & 1);
-      const s16x4 lo = read_transposed(vt + (r0 * L::VP + (piece ^ L::v_swizzle(r0))) * 16 + in);
-      const s16x4 hi = read_transposed(vt + ((r0 + 8) * L::VP + (piece ^ L::v_swizzle(r0 + 8))) * 16 + in);
-      return join<v8>(lo, hi);
-    };
-    auto k_operand = [&](int i, int u) {
-      const int r = 32 * i + (ln & 31);
-      return *reinterpret_cast<const v8*>(kt + (r * L::KP + ((2 * u + lh) ^ L::k_swizzle(r))) * 16);
-    };
-    constexpr int AHEAD = VT < 4 ? VT : 4, KS = D / 16;                // products whose operands are on their way; products of a group of keys
-    v8 kf[AHEAD], vf[AHEAD];
+  auto request_v = [&](int g) {
+    if (g < groups) request_group_v<T, D, 2 * RG>(a, v + (int64_t)g * L::KEYS * a.vs[1], n.k - 1 - g * L::KEYS, lds_at + g % L::SLOTS * L::BYTES);
+  };
+  auto v_operand = [&](const char* vt, int ln, int u, int t) {         // k slot (h, e) of step u holds key 16 u + 8 (e / 4) + 4 h + e % 4: the accumulator layout of S^T
+    const int r0 = 16 * u + 4 * (ln >> 5) + ((ln & 15) >> 2), piece = 4 * t + 2 * ((ln >> 4) & 1) + ((ln & 3) >> 1), in = 8 * (ln & 1);
+    const s16x4 lo = read_transposed(vt + (r0 * L::VP + (piece ^ L::v_swizzle(r0))) * 16 + in);
+    const s16x4 hi = read_transposed(vt + ((r0 + 8) * L::VP + (piece ^ L::v_swizzle(r0 + 8))) * 16 + in);
+    return join<v8>(lo, hi);
+  };
+  auto k_operand = [&](const char* kt, int ln, int i, int u) {
+    const int r = 32 * i + (ln & 31);
+    return *reinterpret_cast<const v8*>(kt + (r * L::KP + ((2 * u + (ln >> 5)) ^ L::k_swizzle(r))) * 16);
+  };
+  f32x16 s[J];
+  v8 pf[2 * J];
+  // The scores of a group.  The next AHEAD operands are always on their way, each requested right behind the product that frees its registers: LDS answers in the time of
+  // several products (8192 x 8192, d = 128: 431 us with 4 ahead in bunches of 4, 427 with 8 in bunches, 412 with 8 in pairs)
+  auto scores = [&](int g, int ln) {
+    const char* kt = lds + g % L::SLOTS * L::BYTES + map * (L::K_BYTES / 2);
+    v8 kf[AHEAD];
 #pragma unroll
-    for (int p = 0; p < AHEAD; ++p) kf[p] = k_operand(p / KS, p % KS);
+    for (int p = 0; p < AHEAD; ++p) kf[p] = k_operand(kt, ln, p / KS, p % KS);
 #pragma unroll
-    for (int j0 = 0; j0 < 2; j0 += J) {
-      f32x16 s[J];
+    for (int i = 0; i < J; ++i) s[i] = f32x16{0};
 #pragma unroll
-      for (int i = 0; i < J; ++i) s[i] = f32x16{0};
-#pragma unroll
-      for (int p = 0; p < J * KS; ++p) {
-        s[p / KS] = Mat<T>::mma32(kf[p % AHEAD], qf[p % KS], s[p / KS]);
-        if (p + AHEAD < J * KS) kf[p % AHEAD] = k_operand(j0 + (p + AHEAD) / KS, (p + AHEAD) % KS);
-        if (p % AHEAD == AHEAD - 1) THA4_SCHED_FENCE();
-      }
-      THA4_SCHED_FENCE();
-#pragma unroll
-      for (int t = 0; t < AHEAD; ++t) vf[t] = v_operand(2 * j0, t);
-      THA4_SCHED_FENCE();
-      if constexpr (part) {
-#pragma unroll
-        for (int i = 0; i < J; ++i)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int key = k0 + 32 * (j0 + i) + 8 * (r / 4) + 4 * h + r % 4;
-            bool seen = key < limit;
-            if (mask) {
-              seen = seen && mask[(int64_t)min(key, a.k_len - 1) * a.ms[3]];
-              if (r % 4 == 3) THA4_SCHED_FENCE();
-            }
-            s[i][r] = seen ? s[i][r] : -INFINITY;
-          }
-      }
-      float top = s[0][0];
-#pragma unroll
-      for (int i = 0; i < J; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
-      top = both_halves(top, Max());
-      // The reference point of the exponents follows the maximum only when that has outgrown it by 2^8 (in the first tiles of nearly every row, seldom later): weights stay below 2^8, which
-      // fp16 and bf16 hold with their full precision, and the accumulator is left alone in most steps
-      const float now = top > m + a.slack ? top : m;
-      if (__any(now != m)) {
-        const float w = now == -INFINITY ? 1.0f : exp2_((m - now) * a.c);
-        l *= w;
-#pragma unroll
-        for (int t = 0; t < VT; ++t) acc[t] *= w;
-        m = now;
-      }
-      const float mc = m == -INFINITY ? 0.0f : m * a.c;
-      v8 pf[2 * J];
-#pragma unroll
-      for (int i = 0; i < J; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float p = exp2_(fmaf(s[i][r], a.c, -mc));
-          l += p;
-          pf[2 * i + r / 8][r % 8] = (T)p;
-        }
-      THA4_SCHED_FENCE();
-#pragma unroll
-      for (int p = 0; p < 2 * J * VT; ++p) {
-        acc[p % VT] = Mat<T>::mma32(vf[p % AHEAD], pf[p / VT], acc[p % VT]);
-        const int next = p + AHEAD;
-        if (next < 2 * J * VT) vf[p % AHEAD] = v_operand(2 * j0 + next / VT, next % VT);
-        if (p % AHEAD == AHEAD - 1) THA4_SCHED_FENCE();
-      }
-      if (j0 + J < 2) {
-#pragma unroll
-        for (int p = 0; p < AHEAD; ++p) kf[p] = k_operand(j0 + J, p);
-      }
+    for (int p = 0; p < J * KS; ++p) {
+      s[p / KS] = Mat<T>::mma32(kf[p % AHEAD], qf[p % KS], s[p / KS]);
+      if (p + AHEAD < J * KS) kf[p % AHEAD] = k_operand(kt, ln, (p + AHEAD) / KS, (p + AHEAD) % KS);
+      if (p % 2) THA4_SCHED_FENCE();
     }
   };
-  int k0 = 0;
-  for (; k0 + kKeys <= wg_full; k0 += kKeys) tile(k0, std::false_type());
-  for (; k0 < wg_end; k0 += kKeys) tile(k0, std::true_type());
+  auto add_values = [&](int g, int ln) {
+    const char* vt = lds + g % L::SLOTS * L::BYTES + L::K_BYTES;
+    v8 vf[AHEAD];
+#pragma unroll
+    for (int p = 0; p < AHEAD; ++p) vf[p] = v_operand(vt, ln, p / VT, p % VT);
+#pragma unroll
+    for (int p = 0; p < 2 * J * VT; ++p) {
+      acc[p % VT] = Mat<T>::mma32(vf[p % AHEAD], pf[p / VT], acc[p % VT]);
+      const int next = p + AHEAD;
+      if (next < 2 * J * VT) vf[p % AHEAD] = v_operand(vt, ln, next / VT, next % VT);
+      if (p % 2) THA4_SCHED_FENCE();
+    }
+  };
+  auto softmax = [&]() {
+    float top = s[0][0];
+#pragma unroll
+    for (int i = 0; i < J; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
+    top = both_halves(top, Max());
+    // The reference point of the exponents follows the maximum only when that has outgrown it by 2^8 (in the first groups of nearly every row, seldom later): weights stay below 2^8, which
+    // fp16 and bf16 hold with their full precision, and the accumulator is left alone in most groups (8192 x 8192, d = 128: 462 -> 443 us)
+    const float now = top > m + a.slack ? top : m;
+    if (__any(now != m)) {
+      const float w = now == -INFINITY ? 1.0f : exp2_((m - now) * a.c);
+      l *= w;
+#pragma unroll
+      for (int t = 0; t < VT; ++t) acc[t] *= w;
+      m = now;
+    }
+    const float mc = m == -INFINITY ? 0.0f : m * a.c;
+#pragma unroll
+    for (int i = 0; i < J; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = exp2_(fmaf(s[i][r], a.c, -mc));
+        l += p;
+        pf[2 * i + r / 8][r % 8] = (T)p;
+      }
+  };
+
+  // Whole groups in phases.  In phase 2 i the first map's waves multiply (values of group i - 1, scores of group i) while the second's take the softmax of group i - 1; in phase 2 i + 1
+  // the other way round.  K of a group is read in phases 2 i and 2 i + 1, V in 2 i + 2 and 2 i + 3; so at the head of phase 2 i the slots of K (i - 1) and V (i - 2) are free
+  // and take K (i + 3) and V (i + 2), and behind phase 2 i + 1 K (i + 1) and V (i) have to be there: everything but the two newest batches.
+  auto batch = [&](int i) { request_k(i + 3); request_v(i + 2); };
+  auto even_end = [&]() { THA4_SCHED_FENCE(); THA4_BARRIER_LDS(); THA4_SCHED_FENCE(); };
+  auto odd_end = [&](int i) { THA4_SCHED_FENCE(); THA4_BARRIER_KEEP(i + 3 < groups ? 2 * BATCH : 0); THA4_SCHED_FENCE(); };
+  request_k(0);
+  request_k(1); request_v(0);
+  request_k(2); request_v(1);
+  if (whole > 0) {
+    odd_end(-1);
+    if (map == 1) { batch(0); even_end(); }
+    for (int i = 0; i <= whole; ++i) {
+      if (map == 0) batch(i);
+      if (i > 0) add_values(i - 1, lane);
+      if (i < whole) scores(i, lane);
+      if (map == 0) even_end(); else odd_end(i);
+      if (i < whole) {
+        if (map == 1) batch(i + 1);
+        softmax();
+      }
+      if (map == 0) odd_end(i); else if (i < whole) even_end();
+    }
+  } else {
+    batch(0);
+  }
+  // Groups that some query sees only a part of, in step
+  for (int g = whole; g < groups; ++g) {
+    THA4_BARRIER_KEEP(0);                                              // this group is there, and everybody has left the one before
+    if (g > whole) request_k(g + 3);
+    request_v(g + 3);
+    quarantine<T, D, 128 * RG>(a, lds + g % L::SLOTS * L::BYTES + L::K_BYTES, acc, g * L::KEYS, limit, mask, &flag);
+    int ln = lane;
+    asm volatile("" : "+v"(ln));                                       // (addresses computed here: kept from the kernel's head they would cost the loop above registers)
+    scores(g, ln);
+#pragma unroll
+    for (int i = 0; i < J; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int key = g * L::KEYS + 32 * i + 8 * (r / 4) + 4 * h + r % 4;
+        bool seen = key < limit;
+        if (mask) {
+          seen = seen && mask[(int64_t)min(key, a.k_len - 1) * a.ms[3]];
+          if (r % 4 == 3) THA4_SCHED_FENCE();
+        }
+        s[i][r] = seen ? s[i][r] : -INFINITY;
+      }
+    softmax();
+    THA4_SCHED_FENCE();
+    add_values(g, ln);
+  }
 
   l = both_halves(l, Add());
   float* meet = reinterpret_cast<float*>(lds) + (wave % RG) * (VT * 16 * 64) + lane;
@@ -524,9 +574,8 @@ __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArg
     if (next < end) wait_copies<L::K_COPIES>();                          // V is here, the next K may be on its way
     else wait_copies<0>();
     if (part) {                                                          // infinities and NaN that a row does not see (see quarantine above)
-      auto finite16 = [](unsigned short u) { return std::is_same<T, bf16>::value ? (u & 0x7f80) != 0x7f80 : (u & 0x7c00) != 0x7c00; };
       bool bad = false;
-      for (int p = lane; p < L::V_COPIES * 512; p += 64) bad |= !finite16(reinterpret_cast<const unsigned short*>(vt)[p]);
+      for (int p = lane; p < L::V_COPIES * 64; p += 64) bad |= not_finite<T>(reinterpret_cast<const u32x4*>(vt)[p]);
       if (__any(bad)) {
         for (int key = 0; key < kTurn; ++key) {
           const bool seen = k0 + key < limit && (!mask || mask[(int64_t)(k0 + key) * a.ms[3]]);
@@ -538,14 +587,11 @@ __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArg
             for (int e = 0; e < 4; ++e) {
               const int dv = 16 * t + 4 * gg + e;
               const T val = reinterpret_cast<const T*>(vt + key * L::VP * 16)[8 * ((dv / 8) ^ L::v_swizzle(key)) + dv % 8];
-              if (seen && !finite16(__builtin_bit_cast(unsigned short, val))) { acc[0][t][e] += (float)val; acc[1][t][e] += (float)val; }
+              if (seen && not_finite(val)) { acc[0][t][e] += (float)val; acc[1][t][e] += (float)val; }
             }
         }
         wait_reads();
-        for (int p = lane; p < L::V_COPIES * 512; p += 64) {
-          unsigned short* u = reinterpret_cast<unsigned short*>(vt) + p;
-          if (!finite16(*u)) *u = 0;
-        }
+        clear_not_finite<T>(vt, L::V_COPIES * 1024, lane, 64);
         wait_reads();
       }
     }
