@@ -42,7 +42,7 @@ int bad(const char* msg) { return fail(THA4_ERR_INVALID_ARGUMENT, msg); }
 
 template <class K, class A>
 int launch(K kernel, int64_t grid, int64_t grid_y, int threads, const A& a, void* stream) {
-  if (grid > kMaxGrid || grid_y > 65535) return bad("too many rows for one launch");
+  if (grid * threads > 0xffffffffLL || grid_y > 65535) return bad("too many rows for one launch");      // (a launch has fewer than 2^32 threads in a direction)
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid, (unsigned)grid_y), dim3(threads), 0, static_cast<hipStream_t>(stream), a);
   HIP_TRY(hipGetLastError());
   return THA4_OK;

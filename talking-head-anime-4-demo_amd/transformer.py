@@ -128,20 +128,18 @@ def int8_linear(x: Tensor, weight: Tensor, weight_scale: Tensor, *, x_scale: Opt
 
 
 def _per_row(t: Tensor, name: str, shape, cols: int, rows: int) -> Tuple[Tensor, int, int]:
-    """A vector [c], a tensor [samples, c] / [samples, 1, .., c] or a full [..., c] -> (its rows, their stride, rows of the input for each)."""
+    """A gate or FiLM tensor -> (its rows, their stride, rows of the input for each): one row ([c], [1, .., c]), a row for each sample ([samples, c],
+    [samples, 1, .., c]; for a two-dimensional input any number of consecutive equal shares) or for each token (the input's shape, or [rows, c])."""
+    if t.shape == shape:
+        return _rows(t, cols) + (1,)
     if t.dim() < 1 or t.shape[-1] != cols:
         raise AssertionError(f"{name} must be [..., {cols}]")
-    if t.shape != shape and t.dim() > 2 and math.prod(t.shape[1:-1]) == 1:
-        t = t.reshape(t.shape[0], cols)
     have = t.numel() // cols
-    t, stride = _rows(t, cols)
-    if have == rows:
-        return t, stride, 1
-    if have == 1:
-        return t, stride, _ONE_ROW
-    if have < 1 or rows % have or not (have == shape[0] or len(shape) == 2):
+    lead = t.shape[0] if t.dim() > 1 else 1
+    if have != lead or (have not in (1, rows, shape[0]) and (len(shape) != 2 or have < 1 or rows % have)):
         raise AssertionError(f"{name} must have one row, one for each sample or one for each token")
-    return t, stride, rows // have
+    t, stride = _rows(t.reshape(have, cols), cols)
+    return t, stride, _ONE_ROW if have == 1 else max(rows // have, 1)
 
 
 def residual_norm(residual: Tensor, branch: Optional[Tensor] = None, *, gate: Optional[Tensor] = None, gate_activation: str = "none",
@@ -230,7 +228,9 @@ def _heads(t: Tensor) -> Tuple[Tensor, Tuple[int, int, int]]:
     if t.is_contiguous():
         if t.data_ptr() % 16:
             t = t.clone()
-    elif t.stride(3) != 1 or t.data_ptr() % 16 or any(s % 8 for s, n in zip(t.stride()[:3], t.shape) if n > 1):
+        _, n, h, d = t.shape
+        return t, (n * h * d, h * d, d)             # (its own strides say nothing where a dimension has one entry)
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s % 8 for s, n in zip(t.stride()[:3], t.shape) if n > 1):
         t = t.contiguous()
     return t, tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape))
 

@@ -172,6 +172,15 @@ def test_residual_norm_options():
     within(y, want[1])
     h, y = transformer.residual_norm(x[:0], x[:0])
     assert h.shape == (0, 40, 256)
+    # what would mean a row for each token of every sample is not taken for a row for each sample
+    two = randn(g, 2, 2, c)
+    with pytest.raises(AssertionError, match="one row"):
+        transformer.residual_norm(two, two, gate=randn(g, 1, 2, c))
+    with pytest.raises(AssertionError, match="one row"):
+        transformer.residual_norm(two, two, film=(randn(g, 1, 2, c), randn(g, 1, 2, c)))
+    for gate in (randn(g, 2, c), randn(g, 1, 1, c), randn(g, 4, c)):
+        h, y = transformer.residual_norm(two, two, gate=gate)
+        within(h, oracle.residual_norm(two, two, gate=gate)[0])
     # rows do not touch each other: an infinity or a NaN stays in its row; a row of zeros has no variance
     x = randn(g, 12, 512)
     b = randn(g, 12, 512)
@@ -324,6 +333,9 @@ def test_attention_strided_views(q_len):
     odd = torch.empty(fused.numel() + 1, dtype=BF16, device="cuda:0")[1:].view_as(fused).copy_(fused)      # 2-byte aligned: copied first
     qo = odd[:, :q_len, :2 * heads * d].unflatten(2, (2 * heads, d))
     within(transformer.differential_attention(qo, k, v, lam, 0.5, causal=True, norm_weight=w), want)
+    odd = torch.empty(1, 1, 2 * heads * d + 3, dtype=BF16, device="cuda:0").expand(1, 1, -1)[..., :2 * heads * d]       # one token of a row of odd length
+    one = odd.unflatten(2, (2 * heads, d)).copy_(q[:1, :1])
+    within(transformer.differential_attention(one, k[:1], v[:1], lam, 0.5, norm_weight=w), oracle.differential_attention(one, k[:1], v[:1], lam, 0.5, norm_weight=w))
     out = torch.empty(2, heads, q_len, 2 * d, dtype=BF16, device="cuda:0").transpose(1, 2)
     within(transformer.differential_attention(q, k, v, lam, 0.5, causal=True, norm_weight=w, out=out), want)
 
@@ -500,3 +512,45 @@ def test_refusals_on_the_device():
     v = torch.zeros(1, 1, 1, 128, dtype=F16, device="cuda:0")
     with pytest.raises(_capi.Tha4Error, match="scale"):
         transformer.differential_attention(q, q, v, torch.zeros(4, 64, device="cuda:0"), 0.5, scale=-1.0)
+
+
+TWIN_CODE = r'''
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+import tha4_amd
+from tha4_amd import transformer as T
+g = torch.Generator(device="cuda:0").manual_seed(21)
+r = lambda *s, dtype=torch.bfloat16: torch.empty(s, device="cuda:0").normal_(generator=g).to(dtype)
+i8 = lambda *s: torch.randint(-127, 128, s, device="cuda:0", generator=g).to(torch.int8)
+out = []
+for m, n, k in ((1, 512, 4096), (16, 16384, 1024), (30, 8192, 1024), (100, 300, 2048), (1024, 1280, 512), (1000, 4096, 1024), (3000, 5000, 640), (200, 257, 333)):
+    out.append(T.int8_linear(r(m, k), i8(n, k), r(n, dtype=torch.float32)))
+for rows, c in ((3, 256), (5, 1024), (9, 4096), (3, 8192), (2, 16384), (4, 77)):
+    out += T.residual_norm(r(rows, c), r(rows, c), gate=r(rows, c), gate_activation="sigmoid", post_norm="layer")
+for d in (32, 64, 128):
+    lam = r(4, d, dtype=torch.float32) * 0.1
+    for b, q, kl, h, kv in ((1, 700, 700, 2, 1), (16, 300, 300, 8, 8), (2, 1, 3000, 4, 1), (1, 1, 70000, 8, 2), (3, 40, 1000, 2, 2)):
+        n = torch.randint(0, kl + 1, (b,), device="cuda:0", generator=g).to(torch.int32)
+        Q, K, V = r(b, q, 2 * h, d), r(b, kl, 2 * kv, d), r(b, kl, kv, 2 * d)
+        out += [T.differential_attention(Q, K, V, lam, 0.5, causal=True), T.differential_attention(Q, K, V, lam, 0.5, kv_lengths=n)]
+torch.cuda.synchronize()
+torch.save([o.cpu() for o in out], sys.argv[2])
+'''
+
+
+def test_same_bits_as_the_forced_wait_twin(tmp_path):
+    """The library whose every wait waits for everything (csrc/libtha4_hip_wait0.so) computes the same bits: no copy, LDS read or matrix result is used before it is there."""
+    import os
+    import subprocess
+    import sys
+    from tha4_amd import _build
+    if not os.path.exists(_build.TWIN) or os.path.getmtime(_build.TWIN) < os.path.getmtime(_build.LIB):
+        pytest.skip("forced-wait twin not built, or older than the library")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    got = []
+    for lib in (_build.LIB, _build.TWIN):
+        to = str(tmp_path / os.path.basename(lib)) + ".pt"
+        done = subprocess.run([sys.executable, "-c", TWIN_CODE, root, to], env=dict(os.environ, THA4_HIP_LIB=lib), capture_output=True, text=True, timeout=110)
+        assert done.returncode == 0, done.stderr[-2000:]
+        got.append(torch.load(to, weights_only=True))
+    assert len(got[0]) == len(got[1]) and all(torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)) for a, b in zip(*got))
