@@ -121,7 +121,13 @@ struct Plan {
 Plan plan_of(const tha4_diff_attention_args& a) {
   Plan p{};
   const int64_t rows = (int64_t)a.q_len * (a.heads / a.kv_heads);
-  p.few = rows <= kRows;
+  // A prompt's workgroup walks through all the keys alone (3.5e-4 us a key and channel: 128 x 8192, d = 64: 189 us however few queries there are); the path for few queries divides
+  // the keys but repeats them for every 16 rows (300 TFLOP/s and two launches).  It is taken where it is clearly the shorter (prompt path / few path, us):
+  // 128 x 8192, 8 heads, d = 64: 189 / 33;  64 x 32768, 8 on 2 heads, d = 128: 1281 / 100;  512 x 4096, 8 heads, d = 64: 98 / 57;  512 x 512: 21 / 32;  1024 x 8192, 8 heads, d = 128: 334 / 320
+  const double keys_d = (double)a.k_len * a.head_dim;
+  const double prompt_us = 3.5e-4 * keys_d * (double)ceil_div((int64_t)a.batch * a.heads * ceil_div(a.q_len, 128), 256);
+  const double few_us = 16.0 + 12.0 / 3e8 * keys_d * (double)a.batch * a.kv_heads * (double)(ceil_div(rows, kRows) * kRows);
+  p.few = rows <= kRows || 1.3 * few_us < prompt_us;
   p.splits = 1;
   p.chunk = a.k_len;
   if (!p.few) return p;
@@ -153,8 +159,10 @@ template <class T, int D>
 int attention(AttnArgs& a, const Plan& p, void* stream) {
   if (!p.few) {
     const int64_t heads = (int64_t)a.batch * a.heads;
-    if (heads * ceil_div(a.q_len, 128) >= 256) return launch(diff_prompt_kernel<T, D, 4>, heads * ceil_div(a.q_len, 128), 1, 512, a, stream);
-    return launch(diff_prompt_kernel<T, D, 2>, heads * ceil_div(a.q_len, 64), 1, 256, a, stream);      // (few queries: workgroups of 64 fill more of the 256 CUs)
+    // d = 32: workgroups of 64 queries where those of 128 leave CUs without one (8 frames of 256 tokens: 10.4 us against 12.8; at d = 64 the wider ones are as fast or faster)
+    if constexpr (D == 32)
+      if (heads * ceil_div(a.q_len, 128) < 256) return launch(diff_prompt_kernel<T, D, 2>, heads * ceil_div(a.q_len, 64), 1, 256, a, stream);
+    return launch(diff_prompt_kernel<T, D, 4>, heads * ceil_div(a.q_len, 128), 1, 512, a, stream);
   }
   const int64_t tiles = (int64_t)a.batch * a.kv_heads * p.row_tiles;
   const int st = launch(diff_few_kernel<T, D>, tiles * p.splits, 1, 256, a, stream);

@@ -136,6 +136,8 @@ def test_workspace_is_a_function_of_the_sizes(lib):
     n = lib.tha4_diff_attention_workspace(a)
     assert n > 0 and n == lib.tha4_diff_attention_workspace(a)
     assert lib.tha4_diff_attention_workspace(attention_args(None, q_len=512, k_len=512)) == 0
+    assert lib.tha4_diff_attention_workspace(attention_args(None, q_len=64, k_len=32768, head_dim=128)) > 0      # few prompts' workgroups over many keys: divided, too
+    assert lib.tha4_diff_attention_workspace(attention_args(None, q_len=8192, k_len=8192, heads=64, kv_heads=64)) == 0
 
 
 def test_python_refuses_cpu_tensors_and_wrong_shapes(lib):

@@ -213,7 +213,7 @@ def attention_inputs(g, batch, q_len, k_len, heads, kv_heads, d, dtype, per_head
 
 ATTENTION = [  # batch, q_len, k_len, heads, kv_heads
     (1, 1, 1, 1, 1), (2, 1, 33, 4, 1), (3, 1, 700, 8, 2), (1, 1, 5000, 4, 4), (2, 4, 1300, 4, 1), (1, 16, 16, 2, 2), (1, 17, 40, 1, 1), (2, 5, 64, 8, 2),
-    (1, 128, 128, 2, 1), (2, 129, 257, 2, 2), (1, 300, 300, 4, 2), (1, 64, 1000, 2, 1), (1, 257, 31, 2, 2), (8, 256, 256, 8, 8), (1, 40, 9000, 1, 1), (3, 70, 0, 2, 1), (2, 3, 0, 2, 1)]
+    (1, 128, 128, 2, 1), (2, 129, 257, 2, 2), (1, 300, 300, 4, 2), (1, 64, 1000, 2, 1), (1, 100, 9000, 3, 1), (2, 33, 5000, 4, 1), (1, 257, 31, 2, 2), (8, 256, 256, 8, 8), (1, 40, 9000, 1, 1), (3, 70, 0, 2, 1), (2, 3, 0, 2, 1)]
 
 
 @pytest.mark.parametrize("d", [32, 64, 128])
@@ -229,7 +229,7 @@ def test_attention(case, dtype, d):
 
 
 @pytest.mark.parametrize("d", [32, 64, 128])
-@pytest.mark.parametrize("q_len", [1, 3, 150])
+@pytest.mark.parametrize("q_len", [1, 3, 150, 1000])
 def test_attention_lengths(q_len, d):
     """Caches of their own lengths: empty, one key, inside and at the end of a tile, full; what lies behind is NaN."""
     g = rng(q_len + d)
@@ -270,7 +270,7 @@ def test_attention_padded_batch(d):
 
 
 @pytest.mark.parametrize("d", [32, 64, 128])
-@pytest.mark.parametrize("q_len,k_len", [(1, 300), (4, 1200), (200, 130)])
+@pytest.mark.parametrize("q_len,k_len", [(1, 300), (4, 1200), (200, 130), (50, 6000)])
 def test_attention_mask(q_len, k_len, d):
     g = rng(q_len + k_len + d)
     q, k, v, lam, w = attention_inputs(g, 2, q_len, k_len, 4, 2, d, BF16)
@@ -287,7 +287,7 @@ def test_attention_mask(q_len, k_len, d):
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("d", [32, 64, 128])
-@pytest.mark.parametrize("q_len,k_len,bad", [(200, 200, 150), (3, 90, 88), (4, 1030, 1027)])
+@pytest.mark.parametrize("q_len,k_len,bad", [(200, 200, 150), (3, 90, 88), (4, 1030, 1027), (40, 9000, 8980)])
 def test_values_that_a_query_does_not_see_do_not_reach_it(q_len, k_len, bad, dtype, d):
     g = rng(bad + d)
     q, k, v, lam, w = attention_inputs(g, 2, q_len, k_len, 4, 2, d, dtype)
