@@ -9,6 +9,7 @@ Layout (only what the per-frame poser path needs):
   poser/           mirror of the reference's ``tha4.poser`` interface (Poser ABC, pose-parameter
                    metadata, modes/mode_14.create_poser) on top of the C ABI
   weights.py       reference ``.pt`` state_dict ingest
+  transformer.py   operators of a transformer block over token sequences (int8 product, norms around a block, differential attention)
   sharding.py      frame-parallel multi-GPU driver (one process per GPU, RCCL gather of finished frames)
 """
-__all__ = ["poser", "weights", "sharding"]
+__all__ = ["poser", "weights", "sharding", "transformer"]

@@ -73,9 +73,10 @@ class Tha4ResidualNormArgs(C.Structure):
 
 
 class Tha4DiffAttentionArgs(C.Structure):
+    """(The header's stride arrays are single fields here: filled by position at a third of an array field's cost.)"""
     _fields_ = [(n, C.c_void_p) for n in ("q_dev", "k_dev", "v_dev", "out_dev", "lambda_vectors_dev", "norm_weight_dev", "q_lengths_dev", "kv_lengths_dev",
                                           "mask_dev", "workspace_dev")] + [("workspace_bytes", C.c_int64)] + \
-               [(n, C.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + [("mask_stride", C.c_int64 * 4)] + \
+               [(f"{n}_stride_{i}", C.c_int64) for n in ("q", "k", "v", "out") for i in range(3)] + [(f"mask_stride_{i}", C.c_int64) for i in range(4)] + \
                [(n, C.c_int64) for n in ("lambda_vector_stride", "lambda_head_stride")] + \
                [(n, C.c_int32) for n in ("dtype", "batch", "q_len", "k_len", "heads", "kv_heads", "head_dim", "causal", "norm")] + \
                [(n, C.c_float) for n in ("scale", "lambda_init", "eps")]

@@ -159,7 +159,7 @@ template <class T, int D>
 int attention(AttnArgs& a, const Plan& p, void* stream) {
   if (!p.few) {
     const int64_t heads = (int64_t)a.batch * a.heads;
-    // d = 32: workgroups of 64 queries where those of 128 leave CUs without one (8 frames of 256 tokens: 10.4 us against 12.8; at d = 64 the wider ones are as fast or faster)
+    // d = 32: workgroups of 64 queries where those of 128 leave CUs without one (8 frames of 256 tokens: 10.5 us against 13.4; at d = 64 the wider ones are as fast or faster)
     if constexpr (D == 32)
       if (heads * ceil_div(a.q_len, 128) < 256) return launch(diff_prompt_kernel<T, D, 2>, heads * ceil_div(a.q_len, 64), 1, 256, a, stream);
     return launch(diff_prompt_kernel<T, D, 4>, heads * ceil_div(a.q_len, 128), 1, 512, a, stream);

@@ -106,6 +106,8 @@ THA4_DEV float lambda_of(const AttnArgs& a, int head) {
 //
 // Two waves share a SIMD: one of each map.  A group costs a wave a stretch of matrix products (with V of the group before, then with K of this one) and a stretch of
 // vector arithmetic (the softmax); the two waves run them in opposite phases, a barrier between the phases, so that one's arithmetic runs under the other's products.
+// Measured, causal: 8192 x 8192, 8 heads, d = 128: 408 us, 1010 TFLOP/s (in step, without the phases: 446); 4096 x 4096, 16 heads on 4, d = 64: 132 us, 780 TFLOP/s.  A phase is
+// bound by the latency of its LDS reads and the barrier behind it: about 1500 cycles for 24 products of 32.
 template <int D>
 struct Tile {
   static constexpr int J = D == 128 ? 1 : 2, KEYS = 32 * J, SLOTS = 4;  // 32-key tiles of a group: one where the accumulator leaves no registers for two
@@ -311,21 +313,24 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
   };
 
   if constexpr (RG == 2) {
-    // Four waves, each alone on its SIMD (or beside another workgroup's): no partner to take turns with (8 frames of 256 tokens, d = 32: 10.4 us in step, 14.0 us in phases)
+    // Four waves, each alone on its SIMD (or beside another workgroup's): no partner to take turns with (8 frames of 256 tokens, d = 32: 10.5 us in step, 14.0 us in phases)
 #pragma unroll
     for (int g = 0; g < 3; ++g) { request_k(g); request_v(g); }
-    for (int g = 0; g < groups; ++g) {
+    auto enter = [&](int g) {
       THA4_BARRIER_KEEP(min(2, groups - 1 - g) * BATCH);               // this group is there, and everybody has left the one before
       request_k(g + 3);
       request_v(g + 3);
-      if (g < whole) {
-        scores(g, lane);
-        softmax();
-        THA4_SCHED_FENCE();
-        add_values(g, lane);
-      } else {
-        part_group(g);
-      }
+    };
+    for (int g = 0; g < whole; ++g) {
+      enter(g);
+      scores(g, lane);
+      softmax();
+      THA4_SCHED_FENCE();
+      add_values(g, lane);
+    }
+    for (int g = whole; g < groups; ++g) {
+      enter(g);
+      part_group(g);
     }
   } else {
     // Whole groups in phases.  In phase 2 i the first map's waves multiply (values of group i - 1, scores of group i) while the second's take the softmax of group i - 1; in phase
@@ -408,6 +413,7 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
 // A workgroup owns a range of the keys; its four waves take turns of 32 keys, each with running statistics and LDS of its own and without barriers.  The next turn's K is
 // requested as soon as this turn's has been read into operands, the next V behind the product with this one: a wave always has one of the two in flight,
 // asynchronously and straight into LDS, behind counted waits.  The waves meet in LDS, the ranges in a second launch.
+// Measured: 32 caches of up to 16384 keys, 16 heads on 4, d = 64 (544 MB): 115 us + 6.5 us for the join, 4.7 TB/s;  131072 keys, 8 heads on 2, d = 128 (268 MB): 50 + 8 us, 5.3 TB/s.
 constexpr int kTurn = 32, kRows = 16, kMaxSplits = 512;
 
 template <int D>

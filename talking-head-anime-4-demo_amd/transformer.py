@@ -209,8 +209,9 @@ def residual_norm(residual: Tensor, branch: Optional[Tensor] = None, *, gate: Op
         film_at, shift_at = film_s.data_ptr(), film_t.data_ptr()
     if params is not None and params not in (dtype, torch.float32):
         raise AssertionError("vectors and film must all be float32 or all of branch's type")
-    h = torch.empty(shape, dtype=residual_type, device=residual.device)
-    y = torch.empty(shape, dtype=dtype, device=residual.device)
+    dense = residual.is_contiguous()
+    h = torch.empty_like(residual) if dense else torch.empty(shape, dtype=residual_type, device=residual.device)
+    y = torch.empty_like(residual) if dense and dtype is residual_type else torch.empty(shape, dtype=dtype, device=residual.device)
     r, r_stride = _rows(residual, cols)
     b, b_stride = (None, 0) if branch is None else _rows(branch, cols)
     args = _capi.Tha4ResidualNormArgs(
@@ -295,7 +296,7 @@ def differential_attention(q: Tensor, k: Tensor, v: Tensor, lambda_vectors: Tens
     args = _capi.Tha4DiffAttentionArgs(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lambda_vectors.data_ptr(), None if norm_weight is None else norm_weight.data_ptr(),
         None if q_lengths is None else q_lengths.data_ptr(), None if kv_lengths is None else kv_lengths.data_ptr(), mask_at, None, 0,
-        q_stride, k_stride, v_stride, out_stride, mask_stride, lambda_vectors.stride(0), lambda_vectors.stride(1) if lambda_vectors.dim() == 3 else 0,
+        *q_stride, *k_stride, *v_stride, *out_stride, *mask_stride, lambda_vectors.stride(0), lambda_vectors.stride(1) if lambda_vectors.dim() == 3 else 0,
         _DTYPES[dtype], batch, q_len, k_len, heads, kv_heads, d, causal, norm, d ** -0.5 if scale is None else scale, lambda_init, eps)
     need = lib.tha4_diff_attention_workspace(args)
     if need > 0:

@@ -122,13 +122,30 @@ def test_attention_refuses(lib):
     refused(lib, f(attention_args(p, q_dev=None), None), "NULL")
     refused(lib, f(attention_args(p, k_dev=None), None), "k / v")
     refused(lib, f(attention_args(C.c_void_p(p.value + 2)), None), "aligned")
-    refused(lib, f(attention_args(p, k_stride=(C.c_int64 * 3)(8, 4, 8)), None), "multiples of 8")
-    refused(lib, f(attention_args(p, k_stride=(C.c_int64 * 3)(8, 1 << 24, 8)), None), "2^24")
-    refused(lib, f(attention_args(p, k_stride=(C.c_int64 * 3)(-8, 8, 8)), None), "negative")
+    refused(lib, f(attention_args(p, k_stride_1=4), None), "multiples of 8")
+    refused(lib, f(attention_args(p, k_stride_1=1 << 24), None), "2^24")
+    refused(lib, f(attention_args(p, k_stride_0=-8), None), "negative")
     refused(lib, f(attention_args(p, k_len=1 << 20), None), "workspace")     # few queries over a long cache: its ranges meet in a workspace
     refused(lib, f(attention_args(p), None), "device pointers")
     assert f(attention_args(p, batch=0), None) == 0
     assert f(attention_args(p, q_len=0), None) == 0
+
+
+def test_argument_blocks_have_the_header_s_layout(tmp_path):
+    """Sizes and a late field's offset of the ctypes mirrors against the compiler's."""
+    import os
+    import subprocess
+    from tha4_amd import _build
+    names = {"tha4_linear_i8_args": (_capi.Tha4LinearI8Args, "y_dtype"), "tha4_residual_norm_args": (_capi.Tha4ResidualNormArgs, "eps"),
+             "tha4_diff_attention_args": (_capi.Tha4DiffAttentionArgs, "lambda_init")}
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stddef.h>\n#include <stdio.h>\n#include "tha4_hip.h"\nint main(void) {' +
+                   "".join(f'printf("%zu %zu\\n", sizeof({n}), offsetof({n}, {f}));' for n, (_, f) in names.items()) + "return 0;}\n")
+    exe = str(tmp_path / "layout")
+    subprocess.run(["gcc", "-I", _build.INCLUDE, str(src), "-o", exe], check=True)
+    lines = subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split("\n")
+    for (cls, field), line in zip(names.values(), lines):
+        assert line.split() == [str(C.sizeof(cls)), str(getattr(cls, field).offset)]
 
 
 def test_workspace_is_a_function_of_the_sizes(lib):
