@@ -255,8 +255,8 @@ __global__ void __launch_bounds__(512) linear_few_kernel(LinearArgs a) {
 //  * DMA (aligned rows): STAGES stages of LDS, filled by asynchronous copies up to three stages ahead behind counted waits - one barrier a stage, which both
 //    publishes the next stage and frees this one.  Otherwise rows go through registers, one stage ahead.
 //  * Stages of 128 k: a copy moves whole 128-byte lines (8192^3: stages of 64 k 577 us, of 128 k 531 us, tokens' quantisation included).
-//  * 256 x 256 tiles: 8192^3 in 488 us, 2250 TOP/s, beside 517 us of the library's int8 product without scales.  Matrix pipes 60 % busy at 1.9 - 2.0 GHz (with zeros for operands, which
-//    leave the clock alone, the 64-k version took 457 us instead of 565): power sets the clock, the rest is the wait for LDS in front of a stage's first products.
+//  * 256 x 256 tiles: 8192^3 in 488 us, 2250 TOP/s, beside 490 - 530 us of the library's int8 product without scales.  Matrix pipes 52 % busy by the counters, at 1.9 - 2.0 GHz: power
+//    sets the clock (an earlier form took 620 us on random numbers and 458 on zeros), the rest is the wait for LDS and the barrier at a stage's head.
 //  * Channels are the matrix tile's rows, dealt so that a lane ends with 16 consecutive channels of one token: the result leaves in 16-byte stores.
 __device__ const i32x4 g_zero16 = {0, 0, 0, 0};                              // what a copy reads behind a row's end
 
