@@ -10,7 +10,8 @@
 //
 // Precision: scores, maxima, sums, accumulators, lambda and the norm are fp32.  The weights p are rounded to the inputs' type once, as operands of the product with V: 2^-8 (bf16) or 2^-11 (fp16)
 // relative at most, which the difference of the maps and the norm behind it enlarge by |A1| + lambda |A2| over |A1 - lambda A2| - 0.0010 to 0.0018 of the result's norm
-// with bf16 on random inputs, beside the 0.0017 that rounding the result itself costs.  Two products (weights and their remainders) would take that away for two thirds more matrix work.
+// with bf16 on random inputs, beside the 0.0017 that rounding the result itself costs.  Second products with what the rounding left take that away: single tokens (at most 16 rows a kv head) over a bf16
+// cache have them, for nothing; prompts do not (8192 x 8192, d = 128: 577 us instead of 414; d = 64, padded: 79 instead of 62).
 #pragma once
 #include "transformer_types.h"
 
@@ -33,11 +34,13 @@ struct AttnArgs {
 
 template <class T> struct Mat;
 template <> struct Mat<f16> {
+  static constexpr bool COARSE = false;
   typedef f16x8 v8;
   static THA4_DEV f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
   static THA4_DEV f32x4 mma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct Mat<bf16> {
+  static constexpr bool COARSE = true;         // 8 bits of a weight survive its rounding
   typedef bf16x8 v8;
   static THA4_DEV f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
   static THA4_DEV f32x4 mma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -527,6 +530,7 @@ __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArg
   const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + 2 * kv * a.ks[2];
   const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2];
   const uint8_t* mask = a.mask ? a.mask + b * a.ms[0] + head * a.ms[1] + qi * a.ms[2] : nullptr;
+  const bool remainders = Mat<T>::COARSE && a.row_tiles == 1;            // where the cache is the traffic the second products cost nothing (121.3 us with and without)
   char* kt = lds + wave * L::WAVE_BYTES;
   char* vt = kt + L::K_COPIES * 1024;
   const unsigned kt_at = lds_address(kt), vt_at = lds_address(vt);
@@ -565,7 +569,7 @@ __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArg
       }
     wait_reads();
     if (next < end) request_k<T, D>(a, k + (int64_t)next * a.ks[1], n.k - 1 - next, kt_at);
-    v8 pf[2];
+    v8 pf[2], pr[2];                                                     // weights, and what their rounding left
     const bool part = k0 + kTurn > full;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -602,6 +606,7 @@ __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArg
           const float p = exp2_(fmaf(s[i][j][e], a.c, -mc));
           l[i] += p;
           pf[i][4 * j + e] = (T)p;
+          if constexpr (Mat<T>::COARSE) pr[i][4 * j + e] = (T)(p - (float)(T)p);
         }
     }
     if (next < end) wait_copies<L::K_COPIES>();                          // V is here, the next K may be on its way
@@ -637,6 +642,10 @@ __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArg
       const v8 vf = join<v8>(lo, hi);
       acc[0][t] = Mat<T>::mma16(vf, pf[0], acc[0][t]);
       acc[1][t] = Mat<T>::mma16(vf, pf[1], acc[1][t]);
+      if (remainders) {
+        acc[0][t] = Mat<T>::mma16(vf, pr[0], acc[0][t]);
+        acc[1][t] = Mat<T>::mma16(vf, pr[1], acc[1][t]);
+      }
     }
     wait_reads();
     if (next < end) request_v<T, D>(a, v + (int64_t)next * a.vs[1], n.k - 1 - next, vt_at);

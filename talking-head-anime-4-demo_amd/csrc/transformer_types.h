@@ -96,7 +96,7 @@ THA4_DEV float row_reduce(float v, F f, float* slot, int wave_of_row) {
 // 16 bytes a lane from memory to LDS (base + 16 lane), asynchronous and unknown to the compiler's own wait counting: with copies in flight that it knows of it waits for
 // all of them in front of every LDS read.  The caller orders it: THA4_BARRIER_KEEP, or an explicit vmcnt wait.
 THA4_DEV void copy16_async(const void* from_lane, unsigned lds_base_uniform) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from_lane), "s"(lds_base_uniform) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from_lane), "s"(lds_base_uniform) : "memory", "m0");
 }
 THA4_DEV unsigned lds_address(const void* p) { return (unsigned)(size_t)(const __attribute__((address_space(3))) char*)p; }
 
