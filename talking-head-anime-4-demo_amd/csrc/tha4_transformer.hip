@@ -121,12 +121,13 @@ struct Plan {
 Plan plan_of(const tha4_diff_attention_args& a) {
   Plan p{};
   const int64_t rows = (int64_t)a.q_len * (a.heads / a.kv_heads);
-  // A prompt's workgroup walks through all the keys alone (3.5e-4 us a key and channel: 128 x 8192, d = 64: 189 us however few queries there are); the path for few queries divides
-  // the keys but repeats them for every 16 rows (300 TFLOP/s and two launches).  It is taken where it is clearly the shorter (prompt path / few path, us):
-  // 128 x 8192, 8 heads, d = 64: 189 / 33;  64 x 32768, 8 on 2 heads, d = 128: 1281 / 100;  512 x 4096, 8 heads, d = 64: 98 / 57;  512 x 512: 21 / 32;  1024 x 8192, 8 heads, d = 128: 334 / 320
+  // A prompt's workgroup walks through all the keys alone (4.6e-4 us a key and channel behind 10 us: 128 x 8192, d = 64: 262 us however few queries there are); the path for few queries
+  // divides the keys but repeats them for every 16 rows (290 TFLOP/s behind two launches).  It is taken where it is clearly the shorter (prompt path / few path, us):
+  // 128 x 8192, 8 heads, d = 64: 262 / 35;  64 x 32768, 8 on 2 heads, d = 128: 1813 / 110;  512 x 4096, 8 heads, d = 64: 134 / 61;  1024 x 8192, 8 heads, d = 128: 468 / 367;
+  // 128 x 1024, 8 heads, d = 64: 44 / 17;  8 x 32 x 512, 8 heads, d = 64: 25 / 20;  512 x 512, 8 heads, d = 64: 26 / 32;  24 x 300, 8 heads, d = 32: 12.6 / 16.8
   const double keys_d = (double)a.k_len * a.head_dim;
-  const double prompt_us = 3.5e-4 * keys_d * (double)ceil_div((int64_t)a.batch * a.heads * ceil_div(a.q_len, 128), 256);
-  const double few_us = 16.0 + 12.0 / 3e8 * keys_d * (double)a.batch * a.kv_heads * (double)(ceil_div(rows, kRows) * kRows);
+  const double prompt_us = 10.0 + 4.6e-4 * keys_d * (double)ceil_div((int64_t)a.batch * a.heads * ceil_div(a.q_len, 128), 256);
+  const double few_us = 16.0 + 12.0 / 2.9e8 * keys_d * (double)a.batch * a.kv_heads * (double)(ceil_div(rows, kRows) * kRows);
   p.few = rows <= kRows || 1.3 * few_us < prompt_us;
   p.splits = 1;
   p.chunk = a.k_len;

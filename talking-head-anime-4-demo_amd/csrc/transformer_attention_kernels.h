@@ -8,10 +8,10 @@
 // product with V is free as long as V^T uses the same order, so P never leaves its registers.  V^T operands come from row-major V in LDS by the transposing read
 // ds_read_b64_tr_b16 (four keys of one column a lane).
 //
-// Precision: scores, maxima, sums, accumulators, lambda and the norm are fp32.  The weights p are rounded to the inputs' type once, as operands of the product with V: 2^-8 (bf16) or 2^-11 (fp16)
-// relative at most, which the difference of the maps and the norm behind it enlarge by |A1| + lambda |A2| over |A1 - lambda A2| - 0.0010 to 0.0018 of the result's norm
-// with bf16 on random inputs, beside the 0.0017 that rounding the result itself costs.  Second products with what the rounding left take that away: single tokens (at most 16 rows a kv head) over a bf16
-// cache have them, for nothing; prompts do not (8192 x 8192, d = 128: 577 us instead of 414; d = 64, padded: 79 instead of 62).
+// Precision: scores, maxima, sums, accumulators, lambda and the norm are fp32.  A weight p is an operand of the product with V as the sum of two numbers of the inputs' type, hi and p - hi: off by 2^-16 (bf16)
+// or 2^-22 (fp16) of itself, where one number would be off by 2^-8 or 2^-11 - which the difference of the maps and the norm behind it enlarge by |A1| + lambda |A2| over |A1 - lambda A2|: seven times what
+// the result's own rounding costs where the maps see nearly the same.  The second product of a pair costs nothing where memory or latency bounds (one token over a cache, 8 frames of 256 tokens) and 5 / 3 of the matrix work
+// elsewhere: 8192 x 8192, d = 128: 596 us instead of 412; d = 64, padded: 84 instead of 66.
 #pragma once
 #include "transformer_types.h"
 
@@ -34,13 +34,11 @@ struct AttnArgs {
 
 template <class T> struct Mat;
 template <> struct Mat<f16> {
-  static constexpr bool COARSE = false;
   typedef f16x8 v8;
   static THA4_DEV f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
   static THA4_DEV f32x4 mma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct Mat<bf16> {
-  static constexpr bool COARSE = true;         // 8 bits of a weight survive its rounding
   typedef bf16x8 v8;
   static THA4_DEV f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
   static THA4_DEV f32x4 mma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -54,6 +52,12 @@ template <class V8>
 THA4_DEV V8 join(s16x4 a, s16x4 b) { return __builtin_bit_cast(V8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7)); }
 
 THA4_DEV float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
+// p as the sum of two numbers of the operands' type
+template <class T>
+THA4_DEV void in_two(float p, T& hi, T& lo) {
+  hi = (T)p;
+  lo = (T)(p - (float)hi);
+}
 // f of the values that lanes i and i + 32 hold, in both: v_permlane32_swap of v with itself leaves the lower half's values in one result, the upper half's in the other
 template <class F>
 THA4_DEV float both_halves(float v, F f) {
@@ -113,8 +117,7 @@ THA4_DEV float lambda_of(const AttnArgs& a, int head) {
 //
 // Two waves share a SIMD: one of each map.  A group costs a wave a stretch of matrix products (with V of the group before, then with K of this one) and a stretch of
 // vector arithmetic (the softmax); the two waves run them in opposite phases, a barrier between the phases, so that one's arithmetic runs under the other's products.
-// Measured, causal: 8192 x 8192, 8 heads, d = 128: 408 us, 1010 TFLOP/s (in step, without the phases: 446); 4096 x 4096, 16 heads on 4, d = 64: 132 us, 780 TFLOP/s.  A phase is
-// bound by the latency of its LDS reads and the barrier behind it: about 1500 cycles for 24 products of 32.
+// Measured, causal: 8192 x 8192, 8 heads, d = 128: 607 us (in step, without the phases: 637): 680 TFLOP/s of the 12 d operations a pair that the formula has, 1130 of the 20 d that run.
 template <int D>
 struct Tile {
   static constexpr int J = D == 128 ? 1 : 2, KEYS = 32 * J, SLOTS = 4;  // 32-key tiles of a group: one where the accumulator leaves no registers for two
@@ -190,7 +193,7 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
   typedef Tile<D> L;
   typedef typename Mat<T>::v8 v8;
   constexpr int VT = D / 16;                                           // tiles of 32 value columns
-  constexpr int J = L::J, KS = D / 16, AHEAD = D == 32 ? 4 : 8;        // products of 32 keys with K; operands on their way from LDS
+  constexpr int J = L::J, KS = D / 16, AHEAD = D == 64 ? 8 : 4;        // products of 32 keys with K; operands on their way from LDS
   constexpr int JOIN = RG * VT * 16 * 64 * 4;                          // bytes in which the second maps' results meet the first's
   constexpr int BATCH = L::BYTES / 1024 / (2 * RG);                    // copies of a wave and group
   constexpr int kQueries = 32 * RG;
@@ -238,9 +241,9 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
     return *reinterpret_cast<const v8*>(kt + (r * L::KP + ((2 * u + (ln >> 5)) ^ L::k_swizzle(r))) * 16);
   };
   f32x16 s[J];
-  v8 pf[2 * J];
+  v8 pf[2 * J], pr[2 * J];                                             // weights, and what their rounding left
   // The scores of a group.  The next AHEAD operands are always on their way, each requested right behind the product that frees its registers: LDS answers in the time of
-  // several products (8192 x 8192, d = 128: 431 us with 4 ahead in bunches of 4, 427 with 8 in bunches, 412 with 8 in pairs)
+  // several products (8192 x 8192, d = 128: 607 us with 4 ahead, 609 with 6, which need every register)
   auto scores = [&](int g, int ln) {
     const char* kt = lds + g % L::SLOTS * L::BYTES + map * (L::K_BYTES / 2);
     v8 kf[AHEAD];
@@ -261,11 +264,17 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
 #pragma unroll
     for (int p = 0; p < AHEAD; ++p) vf[p] = v_operand(vt, ln, p / VT, p % VT);
 #pragma unroll
-    for (int p = 0; p < 2 * J * VT; ++p) {
-      acc[p % VT] = Mat<T>::mma32(vf[p % AHEAD], pf[p / VT], acc[p % VT]);
-      const int next = p + AHEAD;
-      if (next < 2 * J * VT) vf[p % AHEAD] = v_operand(vt, ln, next / VT, next % VT);
-      if (p % 2) THA4_SCHED_FENCE();
+    for (int p = 0; p < 2 * J * VT; p += 2) {                          // (two tiles in turn: a product never waits for the one before)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) acc[(p + e) % VT] = Mat<T>::mma32(vf[(p + e) % AHEAD], pf[p / VT], acc[(p + e) % VT]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) acc[(p + e) % VT] = Mat<T>::mma32(vf[(p + e) % AHEAD], pr[p / VT], acc[(p + e) % VT]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int next = p + e + AHEAD;
+        if (next < 2 * J * VT) vf[(p + e) % AHEAD] = v_operand(vt, ln, next / VT, next % VT);
+      }
+      THA4_SCHED_FENCE();
     }
   };
   auto softmax = [&]() {
@@ -275,8 +284,8 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
     top = both_halves(top, Max());
-    // The reference point of the exponents follows the maximum only when that has outgrown it by 2^8 (in the first groups of nearly every row, seldom later): weights stay below 2^8, which
-    // fp16 and bf16 hold with their full precision, and the accumulator is left alone in most groups (8192 x 8192, d = 128: 462 -> 443 us)
+    // The reference point of the exponents follows the maximum only when that has outgrown it by 2^8 (in the first groups of nearly every row, seldom later): the accumulator is left
+    // alone in most groups (8192 x 8192, d = 128, one product a weight: 462 -> 443 us)
     const float now = top > m + a.slack ? top : m;
     if (__any(now != m)) {
       const float w = now == -INFINITY ? 1.0f : exp2_((m - now) * a.c);
@@ -291,8 +300,11 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const float p = exp2_(fmaf(s[i][r], a.c, -mc));
+        T hi, lo;
+        in_two(p, hi, lo);
         l += p;
-        pf[2 * i + r / 8][r % 8] = (T)p;
+        pf[2 * i + r / 8][r % 8] = hi;
+        pr[2 * i + r / 8][r % 8] = lo;
       }
   };
 
@@ -530,7 +542,6 @@ __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArg
   const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + 2 * kv * a.ks[2];
   const T* v = static_cast<const T*>(a.v) + b * a.vs[0] + kv * a.vs[2];
   const uint8_t* mask = a.mask ? a.mask + b * a.ms[0] + head * a.ms[1] + qi * a.ms[2] : nullptr;
-  const bool remainders = Mat<T>::COARSE && a.row_tiles == 1;            // where the cache is the traffic the second products cost nothing (121.3 us with and without)
   char* kt = lds + wave * L::WAVE_BYTES;
   char* vt = kt + L::K_COPIES * 1024;
   const unsigned kt_at = lds_address(kt), vt_at = lds_address(vt);
@@ -604,9 +615,11 @@ __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArg
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float p = exp2_(fmaf(s[i][j][e], a.c, -mc));
+          T hi, lo;
+          in_two(p, hi, lo);
           l[i] += p;
-          pf[i][4 * j + e] = (T)p;
-          if constexpr (Mat<T>::COARSE) pr[i][4 * j + e] = (T)(p - (float)(T)p);
+          pf[i][4 * j + e] = hi;
+          pr[i][4 * j + e] = lo;
         }
     }
     if (next < end) wait_copies<L::K_COPIES>();                          // V is here, the next K may be on its way
@@ -642,10 +655,8 @@ __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArg
       const v8 vf = join<v8>(lo, hi);
       acc[0][t] = Mat<T>::mma16(vf, pf[0], acc[0][t]);
       acc[1][t] = Mat<T>::mma16(vf, pf[1], acc[1][t]);
-      if (remainders) {
-        acc[0][t] = Mat<T>::mma16(vf, pr[0], acc[0][t]);
-        acc[1][t] = Mat<T>::mma16(vf, pr[1], acc[1][t]);
-      }
+      acc[0][t] = Mat<T>::mma16(vf, pr[0], acc[0][t]);
+      acc[1][t] = Mat<T>::mma16(vf, pr[1], acc[1][t]);
     }
     wait_reads();
     if (next < end) request_v<T, D>(a, v + (int64_t)next * a.vs[1], n.k - 1 - next, vt_at);

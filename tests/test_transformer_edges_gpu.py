@@ -1,0 +1,41 @@
+"""Transformer block operators on the device where their promises are hardest to keep: small differences of large maps, weights far below the largest, single kernels of
+the dispatch, the ends of the ranges.  Against the same 64-bit definitions and bounds as test_transformer_gpu.py."""
+import pytest
+import torch
+
+import tha4_amd  # noqa: F401
+from oracle import transformer_oracle as oracle
+from test_transformer_gpu import attention_inputs, randn, rng, within
+from tha4_amd import _capi, transformer
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+@pytest.fixture(scope="module", autouse=True)
+def dev():
+    _capi.load_library()
+    assert any("libtha4_" in l and ".so" in l for l in open("/proc/self/maps").read().splitlines())
+
+
+# ---- attention: the weights' precision -------------------------------------------------------------------------------------------------------
+# One case for each form: prompts with 64 and with 128 queries a workgroup, few queries in one range, in several, and in several row tiles
+FORMS = [(2, 200, 500, 2, 1), (8, 256, 256, 8, 8), (48, 256, 256, 4, 4), (2, 1, 200, 4, 2), (1, 4, 5000, 4, 1), (1, 40, 9000, 1, 1)]
+
+
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("case", FORMS, ids=lambda c: "x".join(map(str, c)))
+def test_a_small_difference_of_the_maps_keeps_its_bits(case, dtype, d):
+    """Maps that see nearly the same, lambda 1: what remains is a tenth of a map and less, where weights of 8 or 11 bits would cost several times the rounding of the result."""
+    g = rng(sum(case) + d)
+    q, k, v, _, _ = attention_inputs(g, *case, d, dtype)
+    for t in (q, k):
+        t[:, :, 1::2] = (0.99 * t[:, :, 0::2].float() + 0.14 * t[:, :, 1::2].float()).to(dtype)
+    lam = torch.zeros(4, d, device="cuda:0")                                     # lambda = lambda_init
+    for causal in (False, True):
+        got = transformer.differential_attention(q, k, v, lam, 1.0, causal=causal, norm=False)
+        want, bound = oracle.differential_attention(q, k, v, lam, 1.0, causal=causal, norm=False)
+        within(got, (want, bound))
+        rounding = (want.to(dtype).double() - want).norm() / want.norm()         # the least an answer of this type can be off
+        assert (got.double() - want).norm() / want.norm() <= 1.05 * rounding
