@@ -110,8 +110,8 @@ def visible(batch, q_len, k_len, causal, q_lengths, kv_lengths, mask, device):
 
 def differential_attention(q, k, v, lambda_vectors, lambda_init, causal=False, q_lengths=None, kv_lengths=None, mask=None, scale=None, norm=True,
                            norm_weight=None, eps=1e-5):
-    """(out, bound).  A weight p is the sum of two numbers of the inputs' type (half(type)^2, and 2^-25
-    absolute where an fp16 weight is subnormal, against a sum of weights of at least 1); scores carry (d + 4) u of sum |q k|; the sums over the keys, both parts' and the weights' own, 3 k_len u."""
+    """(out, bound).  A weight p is the sum of two numbers of the inputs' type (half(type)^2; the fp16 weights are held 2^12 times as large at least, so one that is
+    subnormal there is off by 2^-25 2^-12 of a sum of weights of at least 1); scores carry (d + 4) u of sum |q k|; the sums over the keys, both parts' and the weights' own, 3 k_len u."""
     batch, q_len, heads2, d = q.shape
     k_len, heads, group = k.shape[1], heads2 // 2, heads2 // k.shape[2]
     scale = 1 / math.sqrt(d) if scale is None else scale
@@ -141,7 +141,7 @@ def differential_attention(q, k, v, lambda_vectors, lambda_init, causal=False, q
         ds = torch.where(seen, (d + 6) * U * top, torch.zeros_like(top))
         ds = (ds.amax(-1, keepdim=True) if k_len else torch.zeros_like(m)) + 4 * U * torch.where(m.isfinite(), m.abs(), torch.zeros_like(m))
         rel = half(q.dtype) ** 2 + 2.02 * ds + (3 * k_len + 60) * U
-        small = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+        small = 2.0 ** -37 if q.dtype == torch.float16 else 0.0
         err = torch.matmul(a, vd.abs()) * rel + small * torch.where(l > 0, 1 / l.clamp_min(1e-300), torch.zeros_like(l)) * torch.matmul(seen.double().expand_as(p), vd.abs())
         maps.append(torch.matmul(a, vd))
         errs.append(err)

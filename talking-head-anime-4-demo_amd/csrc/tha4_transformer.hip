@@ -317,7 +317,7 @@ int tha4_diff_attention(const tha4_diff_attention_args* args, void* stream) {
   a.batch = g.batch; a.q_len = g.q_len; a.k_len = g.k_len; a.heads = g.heads; a.kv_heads = g.kv_heads; a.group = g.heads / g.kv_heads;
   a.causal = g.causal; a.norm = g.norm;
   a.row_tiles = p.row_tiles; a.splits = p.splits; a.chunk = p.chunk; a.part_rows = p.part_rows;
-  a.c = g.scale * 1.44269504088896340736f; a.slack = 8.0f / a.c; a.lambda_init = g.lambda_init; a.eps = g.eps;
+  a.c = g.scale * 1.44269504088896340736f; a.slack = (g.dtype == THA4_F16 ? Mat<f16>::SLACK : Mat<bf16>::SLACK) / a.c; a.lambda_init = g.lambda_init; a.eps = g.eps;
   return g.dtype == THA4_F16 ? attention<f16>(a, g.head_dim, p, stream) : attention<bf16>(a, g.head_dim, p, stream);
 }
 

@@ -29,16 +29,20 @@ struct AttnArgs {
   int64_t lambda_vs, lambda_hs;
   int32_t batch, q_len, k_len, heads, kv_heads, group, causal, norm;
   int32_t row_tiles, splits, chunk, part_rows;
-  float c, slack, lambda_init, eps;            // c = scale * log2(e): the softmax is taken in powers of two; slack = 8 / c
+  float c, slack, lambda_init, eps;            // c = scale * log2(e): the softmax is taken in powers of two; slack = SLACK / c
 };
 
+// A weight is held as 2^BIAS p in two parts, hi and what its rounding left.  BIAS: p <= 1 (few queries), p <= 2^SLACK (prompts, whose reference point follows the maximum lazily).  fp16 has no
+// exponents to spare: its weights are raised to just below its largest number (2^15), so that only those below 2^-40 or 2^-37 of the largest lose their last bits to its subnormals.
 template <class T> struct Mat;
 template <> struct Mat<f16> {
+  static constexpr float SLACK = 3.0f, BIAS_PROMPT = 12.0f, BIAS_FEW = 15.0f;
   typedef f16x8 v8;
   static THA4_DEV f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
   static THA4_DEV f32x4 mma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 template <> struct Mat<bf16> {
+  static constexpr float SLACK = 8.0f, BIAS_PROMPT = 0.0f, BIAS_FEW = 0.0f;
   typedef bf16x8 v8;
   static THA4_DEV f32x16 mma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
   static THA4_DEV f32x4 mma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -284,9 +288,9 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
     top = both_halves(top, Max());
-    // The reference point of the exponents follows the maximum only when that has outgrown it by 2^8 (in the first groups of nearly every row, seldom later): the accumulator is left
+    // The reference point of the exponents follows the maximum only when that has outgrown it by 2^SLACK (in the first groups of nearly every row, seldom later): the accumulator is left
     // alone in most groups (8192 x 8192, d = 128, one product a weight: 462 -> 443 us)
-    const float now = top > m + a.slack ? top : m;
+    const float now = top - m > a.slack ? top : m;                      // (the difference: exact where it is small, whatever the size of the scores)
     if (__any(now != m)) {
       const float w = now == -INFINITY ? 1.0f : exp2_((m - now) * a.c);
       l *= w;
@@ -294,12 +298,12 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
       for (int t = 0; t < VT; ++t) acc[t] *= w;
       m = now;
     }
-    const float mc = m == -INFINITY ? 0.0f : m * a.c;
+    const float from = m == -INFINITY ? 0.0f : m;
 #pragma unroll
     for (int i = 0; i < J; ++i)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float p = exp2_(fmaf(s[i][r], a.c, -mc));
+        const float p = exp2_(fmaf(s[i][r] - from, a.c, Mat<T>::BIAS_PROMPT));
         T hi, lo;
         in_two(p, hi, lo);
         l += p;
@@ -609,12 +613,12 @@ __global__ void __launch_bounds__(256, D == 128 ? 1 : 2) diff_few_kernel(AttnArg
         for (int t = 0; t < L::VT; ++t) acc[i][t] *= w;
         m[i] = now;
       }
-      const float mc = m[i] == -INFINITY ? 0.0f : m[i] * a.c;
+      const float from = m[i] == -INFINITY ? 0.0f : m[i];
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float p = exp2_(fmaf(s[i][j][e], a.c, -mc));
+          const float p = exp2_(fmaf(s[i][j][e] - from, a.c, Mat<T>::BIAS_FEW));
           T hi, lo;
           in_two(p, hi, lo);
           l[i] += p;

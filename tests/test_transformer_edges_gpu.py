@@ -1,5 +1,7 @@
 """Transformer block operators on the device where their promises are hardest to keep: small differences of large maps, weights far below the largest, single kernels of
 the dispatch, the ends of the ranges.  Against the same 64-bit definitions and bounds as test_transformer_gpu.py."""
+import math
+
 import pytest
 import torch
 
@@ -39,3 +41,43 @@ def test_a_small_difference_of_the_maps_keeps_its_bits(case, dtype, d):
         within(got, (want, bound))
         rounding = (want.to(dtype).double() - want).norm() / want.norm()         # the least an answer of this type can be off
         assert (got.double() - want).norm() / want.norm() <= 1.05 * rounding
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("gap", [16.0, 18.0, 22.0])
+@pytest.mark.parametrize("q_len,k_len,d", [(1, 256, 64), (1, 131072, 128), (4, 20000, 64), (300, 4096, 64), (300, 4096, 128), (256, 512, 32)])
+def test_a_key_that_takes_all_the_weight_and_gives_nothing(q_len, k_len, d, gap, dtype):
+    """A first key with weight e^gap times the others' and values of zero: the answer is what all the others together contribute."""
+    g = rng(q_len + k_len)
+    q, k, v, _, w = attention_inputs(g, 1, q_len, k_len, 2, 1, d, dtype)
+    v += 0.8
+    q[..., 0] = 8.0
+    k *= 0.7
+    k[..., 0] = 0
+    k[0, 0] = 0
+    k[0, 0, :, 0] = gap * math.sqrt(d) / 8.0
+    v[0, 0] = 0
+    lam = torch.zeros(4, d, device="cuda:0")
+    kw = dict(norm_weight=w, eps=1e-14)
+    want, bound = oracle.differential_attention(q, k, v, lam, 0.25, **kw)
+    got = transformer.differential_attention(q, k, v, lam, 0.25, **kw)
+    within(got, (want, bound))
+    assert float(want.abs().mean()) > 0.1
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("q_len,k_len", [(1, 300), (200, 300), (2, 4000)])
+def test_scores_beyond_the_exponents_of_a_weight(q_len, k_len, dtype):
+    """Scores of 1e6 and more, where a step of the 32-bit score is a factor of the weight: still one key takes everything, and no weight leaves the type's range."""
+    d = 64
+    g = rng(q_len + k_len)
+    q, k, v, lam, _ = attention_inputs(g, 1, q_len, k_len, 2, 1, d, dtype)
+    q[...] = 0
+    k[...] = 0
+    q[..., 0] = 30000.0
+    order = torch.randperm(k_len, device="cuda:0", generator=g)
+    k[0, :, :, 0] = (order.float() * 16)[:, None].to(dtype)                      # products up to 30000 * 16 * 4000; all different, many of them within a rounding of each other's weight
+    k[0, order.argmax(), :, 0] = 65504.0 if dtype == F16 else 2.0 ** 17
+    got = transformer.differential_attention(q, k, v, torch.zeros(4, d, device="cuda:0"), 0.25, norm=False)
+    want = v[0, order.argmax(), 0].double() * 0.75
+    assert (got.double() - want).abs().max() <= 2 * oracle.half(dtype) * want.abs().max()
