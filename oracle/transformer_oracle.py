@@ -149,6 +149,7 @@ def differential_attention(q, k, v, lambda_vectors, lambda_init, causal=False, q
     do = errs[0] + lam.abs() * errs[1] + dlam * maps[1].abs() + 3 * U * (maps[0].abs() + (lam * maps[1]).abs())
     if norm:
         ms = (o * o).mean(-1, keepdim=True)
+        ms = torch.where(ms + eps > 0, ms, torch.ones_like(ms))                  # a row of zeros stays one, also with eps = 0
         g = (1 - lambda_init) / torch.sqrt(ms + eps)
         w = torch.ones(2 * d, dtype=torch.float64, device=q.device) if norm_weight is None else norm_weight.double()
         dms = 2 * (o.abs() * do).mean(-1, keepdim=True) + (do * do).mean(-1, keepdim=True) + (2 * d + 8) * U * ms

@@ -112,6 +112,10 @@ THA4_DEV float lambda_of(const AttnArgs& a, int head) {
   return expf(wave_reduce(s, Add())) - expf(wave_reduce(t, Add())) + a.lambda_init;
 }
 
+// the norm's factor of a row whose squares sum to ss: zero for a row of zeros also where eps is zero (a query that sees no key answers zero)
+template <int D>
+THA4_DEV float norm_factor(const AttnArgs& a, float ss) { return !a.norm ? 1.0f : ss == 0.0f ? 0.0f : (1.0f - a.lambda_init) / sqrtf(ss * (1.0f / (2 * D)) + a.eps); }
+
 // ---- prompts: many queries ---------------------------------------------------------------------------------------------------------------
 // A workgroup owns 32 RG queries of one head: 2 RG waves, wave w the queries 32 (w % RG) .. + 31 of map w / RG (the maps meet once, at the end: each wave carries one
 // map's accumulator, which is what lets 2 x 2d columns fit the registers).  Keys go through LDS in groups, K of both maps and V, through a ring of four groups:
@@ -416,7 +420,7 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
   asm volatile("" : "+v"(le));                                        // (the query's number again: not worth a register throughout the loop)
   const int qi = qw + (le & 31);
   if (qi >= n.q) return;
-  const float g = a.norm ? (1.0f - a.lambda_init) / sqrtf(ss * (1.0f / (2 * D)) + a.eps) : 1.0f;
+  const float g = norm_factor<D>(a, ss);
   T* out = static_cast<T*>(a.out) + b * a.os[0] + qi * a.os[1] + head * a.os[2];
   typedef T T4 __attribute__((ext_vector_type(4)));
 #pragma unroll
@@ -460,8 +464,6 @@ THA4_DEV void store_columns(const AttnArgs& a, T* out, int dv, const f32x4& o, f
   for (int e = 0; e < 4; ++e) r[e] = (T)(o[e] * g * (a.norm && a.norm_w ? a.norm_w[dv + e] : 1.0f));
   *reinterpret_cast<T4*>(out + dv) = r;
 }
-template <int D>
-THA4_DEV float norm_factor(const AttnArgs& a, float ss) { return a.norm ? (1.0f - a.lambda_init) / sqrtf(ss * (1.0f / (2 * D)) + a.eps) : 1.0f; }
 THA4_DEV float weight_of(float top, float l) { return l > 0.0f || l != l ? top / l : 0.0f; }      // (no key seen: nothing)
 
 // out of O1, l1, O2, l2 (accumulator layout: row lane % 16, value columns 16 t + 4 (lane / 16) + e)

@@ -233,3 +233,11 @@ def test_oracle_attention_against_a_direct_statement():
                 o = 0.6 * o / torch.sqrt((o * o).mean() + 1e-5) * w
                 assert torch.allclose(out[b, i, h], o, atol=1e-12)
     assert (bound >= 0).all() and float(bound.max()) < 0.02
+
+
+def test_oracle_attention_of_nothing_is_zero_without_eps():
+    g = torch.Generator().manual_seed(3)
+    q, k, v = torch.randn(2, 4, 2, 32, generator=g).half(), torch.randn(2, 6, 2, 32, generator=g).half(), torch.randn(2, 6, 1, 64, generator=g).half()
+    out, bound = oracle.differential_attention(q, k, v, torch.zeros(4, 32), 0.5, kv_lengths=torch.tensor([0, 6]), eps=0.0)
+    assert not out[0].any() and out[1].abs().min(-1)[0].isfinite().all() and bound.isfinite().all()
+    assert torch.allclose((out[1] ** 2).mean(-1), torch.full((4, 1), 0.25, dtype=torch.float64))

@@ -81,3 +81,22 @@ def test_scores_beyond_the_exponents_of_a_weight(q_len, k_len, dtype):
     got = transformer.differential_attention(q, k, v, torch.zeros(4, d, device="cuda:0"), 0.25, norm=False)
     want = v[0, order.argmax(), 0].double() * 0.75
     assert (got.double() - want).abs().max() <= 2 * oracle.half(dtype) * want.abs().max()
+
+
+# ---- attention: queries that see nothing -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("q_len,k_len", [(1, 200), (3, 6000), (40, 9000), (150, 150), (300, 700), (2, 0), (70, 0)])
+def test_a_query_that_sees_no_key_answers_zero_without_eps(q_len, k_len, d, dtype):
+    """eps = 0: the norm of a row of zeros.  An empty sequence, a head and a row that are masked wholly, no keys at all; one range of keys, several, prompts."""
+    g = rng(q_len + k_len + d)
+    q, k, v, lam, w = attention_inputs(g, 2, q_len, k_len, 4, 2, d, dtype)
+    lengths = torch.tensor([0, k_len], dtype=torch.int32, device="cuda:0")
+    mask = torch.ones(2, 4, q_len, k_len, dtype=torch.bool, device="cuda:0")
+    mask[1, 1], mask[1, 2, q_len // 2] = False, False
+    for causal in (False, True):
+        for kw in (dict(kv_lengths=lengths), dict(mask=mask)):
+            kw.update(causal=causal, norm_weight=w, eps=0.0)
+            got = transformer.differential_attention(q, k, v, lam, 0.5, **kw)
+            within(got, oracle.differential_attention(q, k, v, lam, 0.5, **kw))
+            assert not (got[0] if "mask" not in kw else got[1, :, 1]).any() and not (got[1, q_len // 2, 2].any() and "mask" in kw)
