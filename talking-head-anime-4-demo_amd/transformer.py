@@ -8,7 +8,8 @@ FiLM + residual, reduced-precision matrix products), for sequences of any length
 
 All of them enqueue on ``torch.cuda.current_stream()`` of their tensors' device, never synchronise, and can be captured into a graph.  Wrong arguments raise
 AssertionError here or ``_capi.Tha4Error`` from the C ABI (include/tha4_hip.h); nothing falls back to another implementation.  They are forward
-operators: tensors that require gradients are refused while gradients are enabled.
+operators: tensors that require gradients are refused while gradients are enabled, tensors with a forward-mode tangent always, and so are views whose memory holds
+the negated values (``Tensor.is_neg``).
 """
 from __future__ import annotations
 
@@ -17,6 +18,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _capi
 
@@ -34,14 +36,19 @@ def _check_tensors(first: Tensor, *others: Optional[Tensor]) -> int:
     if not first.is_cuda:
         raise AssertionError("tensors must be on the GPU")
     device = first.get_device()
-    gradient = first.requires_grad
+    gradient, negated = first.requires_grad, first.is_neg()
     for t in others:
         if t is not None:
             if t.get_device() != device:
                 raise AssertionError(f"tensors must be on one GPU: {t.device} and {first.device}")
             gradient = gradient or t.requires_grad
+            negated = negated or t.is_neg()
+    if negated:
+        raise AssertionError("a tensor's memory holds its values negated (a view of a complex conjugate): pass tensor.resolve_neg()")
     if gradient and torch.is_grad_enabled():
         raise AssertionError("an input requires a gradient: this is a forward operator (use torch.no_grad())")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in (first,) + others):
+        raise AssertionError("an input carries a forward-mode tangent: this operator has no derivative (use unpack_dual(tensor).primal)")
     return device
 
 

@@ -100,3 +100,46 @@ def test_a_query_that_sees_no_key_answers_zero_without_eps(q_len, k_len, d, dtyp
             got = transformer.differential_attention(q, k, v, lam, 0.5, **kw)
             within(got, oracle.differential_attention(q, k, v, lam, 0.5, **kw))
             assert not (got[0] if "mask" not in kw else got[1, :, 1]).any() and not (got[1, q_len // 2, 2].any() and "mask" in kw)
+
+
+# ---- tensors whose memory is not all they are ------------------------------------------------------------------------------------------------
+def calls(dtype=BF16):
+    """(name, function, its tensor arguments by name): one call of each operator with everything that it can be given."""
+    g = rng(11)
+    x, c = randn(g, 6, 64, dtype=dtype), randn(g, 64)
+    w = transformer.quantize_tokens(randn(g, 32, 64))
+    q, k, v, lam, nw = attention_inputs(g, 2, 3, 40, 2, 1, 32, dtype)
+    return [("quantize", transformer.quantize_tokens, dict(x=x)),
+            ("linear", transformer.int8_linear, dict(x=x, weight=w[0], weight_scale=w[1], bias=randn(g, 32))),
+            ("linear int8", lambda **a: transformer.int8_linear(w[0], out_dtype=F32, **a), dict(weight=w[0], weight_scale=w[1], x_scale=w[1], bias=randn(g, 32))),
+            ("norm", lambda film_scale, film_shift, **a: transformer.residual_norm(film=(film_scale, film_shift), post_norm="layer", pre_norm="layer", **a),
+             dict(residual=x, branch=x + 1, gate=x * 2, residual_scale=c, post_weight=c + 1, post_bias=c + 2, pre_weight=c + 3, pre_bias=c + 4, film_scale=randn(g, 2, 64), film_shift=randn(g, 2, 64))),
+            ("attention", lambda **a: transformer.differential_attention(lambda_init=0.5, **a),
+             dict(q=q, k=k, v=v, lambda_vectors=lam, norm_weight=nw, out=torch.empty(2, 3, 2, 64, dtype=dtype, device="cuda:0")))]
+
+
+def negated_view(t):
+    """A view that holds t's values as the negative of what lies in memory."""
+    v = torch._neg_view(-t)
+    assert v.is_neg() and torch.equal(v, t)
+    return v
+
+
+@pytest.mark.parametrize("at", range(5))
+def test_negated_views_and_forward_mode_tangents_are_refused(at):
+    from torch.autograd import forward_ad
+    name, f, tensors = calls()[at]
+    f(**tensors)
+    for which, t in tensors.items():
+        if not t.is_floating_point():
+            continue
+        with pytest.raises(AssertionError, match="negated"):
+            f(**{**tensors, which: negated_view(t)})
+        f(**{**tensors, which: negated_view(t).resolve_neg()})
+        with forward_ad.dual_level():
+            f(**tensors)                                                         # (a level without tangents changes nothing)
+            with pytest.raises(AssertionError, match="tangent"):
+                f(**{**tensors, which: forward_ad.make_dual(t, torch.ones_like(t))})
+    z = torch.randn(6, 64, dtype=torch.complex64, device="cuda:0").conj()
+    with pytest.raises(AssertionError, match="negated"):
+        transformer.quantize_tokens(z.imag)
