@@ -143,3 +143,55 @@ def test_negated_views_and_forward_mode_tangents_are_refused(at):
     z = torch.randn(6, 64, dtype=torch.complex64, device="cuda:0").conj()
     with pytest.raises(AssertionError, match="negated"):
         transformer.quantize_tokens(z.imag)
+
+
+# ---- the int8 product: every kernel that its rule can choose ---------------------------------------------------------------------------------
+PRODUCTS = [  # m, n, k; rows of w and x 16-byte aligned where k is a multiple of 16
+    (16, 16400, 1024), (5, 16384, 80), (16, 16385, 1040),                        # few tokens, tiles of 64 channels
+    (30, 16400, 512), (17, 16450, 2064),                                         # ... and 32 tokens
+    (30, 8200, 1024), (32, 8193, 48),                                            # tiles of 32 channels x 32 tokens
+    (32, 16401, 1001), (16, 16400, 333),                                         # the same sizes, unaligned
+    (3000, 5000, 640), (3100, 4097, 2064), (3000, 5000, 333),                    # 256 x 256 tiles, aligned and not
+    (1000, 4096, 1024), (1025, 3585, 144), (1000, 4096, 1001),                   # 128 x 128
+    (1024, 1281, 336), (1000, 1300, 1488), (1024, 1281, 333),                    # 64 x 64, one group
+    (33, 65, 16), (257, 1000, 4112), (257, 1000, 4001)]                          # 64 x 64, four groups
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_every_product_kernel_against_the_definition(m, n, k, dtype):
+    g = rng(m + n + k)
+    w, ws = transformer.quantize_tokens(randn(g, n, k))
+    ws = ws * (randn(g, n) * 0.2).exp() / math.sqrt(k)
+    bias = randn(g, n)
+    x = randn(g, m, k, dtype=dtype) * randn(g, m, 1).exp().to(dtype)
+    xq, xs = oracle.quantize(x)
+    got = transformer.int8_linear(x, w, ws, bias=bias)
+    within(got, oracle.int8_linear(xq, xs, w, ws, bias, dtype))
+    assert torch.equal(transformer.int8_linear(xq, w, ws, x_scale=xs, bias=bias, out_dtype=dtype), got)
+    within(transformer.int8_linear(xq, w, ws, x_scale=xs, out_dtype=dtype), oracle.int8_linear(xq, xs, w, ws, None, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("m,n,k", [(3, 130, 1111), (1, 65, 20001), (1, 300, 32768), (1, 33, 32769), (4, 70, 8192), (4, 70, 8193), (2, 100, 4100), (3, 64, 4104), (4, 50, 1), (2, 17, 15)])
+def test_tokens_quantised_inside_the_product(m, n, k, dtype):
+    g = rng(m * n + k)
+    w, ws = transformer.quantize_tokens(randn(g, n, k))
+    bias = randn(g, n)
+    wide = randn(g, m, k + 5, dtype=dtype)
+    for x in (wide[:, :k].contiguous(), wide[:, :k], wide[:, 5:]):               # rows of another stride, at another alignment
+        xq, xs = oracle.quantize(x)
+        within(transformer.int8_linear(x, w, ws / math.sqrt(k), bias=bias), oracle.int8_linear(xq, xs, w, ws / math.sqrt(k), bias, dtype))
+
+
+@pytest.mark.parametrize("m,n", [(1, 64), (20, 130), (33, 65), (600, 520)])
+@pytest.mark.parametrize("k", [131071, 131056])
+def test_the_longest_sums_are_exact(m, n, k):
+    """k = 131071 of the largest products: 2^31 - 16384, and the same negative; scales of one, so the answer is the integer rounded to fp32."""
+    x = torch.full((m, k), -128, dtype=torch.int8, device="cuda:0")
+    w = torch.full((n, k), -128, dtype=torch.int8, device="cuda:0")
+    x[0::2, 77], w[1::2] = 127, 127
+    x[m // 2] = torch.randint(-128, 128, (k,), device="cuda:0", generator=rng(k + m)).to(torch.int8)
+    one = lambda c: torch.ones(c, device="cuda:0")
+    got = transformer.int8_linear(x, w, one(n), x_scale=one(m), out_dtype=F32)
+    assert torch.equal(got, (x.double() @ w.double().t()).float())
