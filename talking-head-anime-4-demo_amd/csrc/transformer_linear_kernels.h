@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(256) quantize_any_kernel(QuantArgs a) {
 
 // ---- product -----------------------------------------------------------------------------------------------------------------------------
 struct LinearArgs {
-  const void* x;               // int8 [m][k], or (linear_token_kernel) the float tokens themselves
+  const void* x;               // int8 [m][k], or (linear_few_kernel<.., INLINE>) the float tokens themselves
   const int8_t* w;
   const float *xs, *ws, *bias;
   void* y;
@@ -147,7 +147,7 @@ THA4_DEV i32x4 piece16(const int8_t* p, int64_t k, int64_t n) {
 // Few tokens: the weights are the traffic.  A workgroup owns 16 NT channels x 16 MT tokens; its 8 waves take turns of 128 k, weights straight from memory into
 // matrix-instruction operands (nothing else would reuse them), AHEAD turns of them on their way at any time, and their exact partial sums meet in LDS.  Every workgroup reads all the tokens, through L2: with 16 of them and one tile of channels that is as much again as the weights.
 // NT tiles for each token operand where there are channels enough to fill the GPU (16 x 16384 x 8192: NT 1 38.9 us, 2 35.6, 4 32.7 = 4.1 TB/s; one token: NT 1 28.1 us = 4.8 TB/s, 4 30.6).
-// INLINE: x is float (XT) and at most kInlineTokens x kInlineK: every workgroup quantises the tokens itself, into LDS, while its first weights are on their
+// INLINE: x is float (XT), m <= kInlineTokens and m k <= kInlineBytes (one token may have 32768 elements): every workgroup quantises the tokens itself, into LDS, while its first weights are on their
 // way - a few hundred instructions against a launch of their own.
 constexpr int kInlineTokens = 4, kInlineBytes = 32768;
 

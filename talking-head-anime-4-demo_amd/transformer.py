@@ -13,7 +13,6 @@ the negated values (``Tensor.is_neg``).
 """
 from __future__ import annotations
 
-import math
 from typing import Optional, Tuple, Union
 
 import torch
