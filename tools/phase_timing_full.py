@@ -20,7 +20,7 @@ if "build" in sys.argv:
     _b = _u.module_from_spec(_sp)
     _sp.loader.exec_module(_b)
     subprocess.run(["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-DTHA4_PHASE_TIMING", *_b.DEVICE_FLAGS, *(["-DTHA4_PHASE_WINDOW"] if "--window" in sys.argv else []), "-I", CSRC, "-I",
-                    os.path.join(ROOT, "include"), os.path.join(CSRC, "tha4_capi.hip"), "-o", lib], check=True)
+                    os.path.join(ROOT, "include"), *(os.path.join(CSRC, s) for s in _b.SOURCES), "-o", lib], check=True)
     sys.exit(0)
 
 import numpy as np

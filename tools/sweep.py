@@ -108,7 +108,7 @@ def build():
         if any("THA4_ABLATE_" in f or "THA4_HUNT_" in f for f in flags):
             base = base + TUNE
         cmd = ["hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-I", CSRC, "-I",
-               os.path.join(ROOT, "include")] + base + flags + [os.path.join(CSRC, "tha4_capi.hip"), "-o", out]
+               os.path.join(ROOT, "include")] + base + flags + [os.path.join(CSRC, s) for s in _bld.SOURCES] + ["-o", out]
         procs.append((name, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)))
     for name, p in procs:
         _, err = p.communicate()
