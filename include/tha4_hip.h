@@ -304,6 +304,7 @@ int tha4_ingest_rgba8(const uint8_t* rgba_dev, int batch, int height, int width,
  * every call can be captured into a graph.  A workspace belongs to one call in flight: two streams, or two captured graphs that may run
  * at once, need one each.  Rows are `cols` contiguous elements, row_stride elements apart.  Outputs must not overlap inputs.
  * Sizes of zero are valid (nothing is written) except where a sum would run over nothing (k, cols, head_dim).
+ * Rows, tokens, channels and sequences that need more workgroups than one launch may have (2^32 threads) are cut into several launches.
  * ------------------------------------------------------------------------------------------------ */
 typedef enum tha4_dtype { THA4_F32 = 0, THA4_F16 = 1, THA4_BF16 = 2 } tha4_dtype;
 

@@ -40,11 +40,25 @@ int one_device(const void* const (&p)[N]) {
 
 int bad(const char* msg) { return fail(THA4_ERR_INVALID_ARGUMENT, msg); }
 
+// A launch has fewer than 2^32 threads in a direction: the most workgroups of one.  What needs more is cut into several launches.
+constexpr int64_t most_workgroups(int threads) { return 0xffffffffLL / threads; }
+
 template <class K, class A>
 int launch(K kernel, int64_t grid, int64_t grid_y, int threads, const A& a, void* stream) {
-  if (grid * threads > 0xffffffffLL || grid_y > 65535) return bad("too many rows for one launch");      // (a launch has fewer than 2^32 threads in a direction)
+  if (grid > most_workgroups(threads) || grid_y > 65535) return bad("too many workgroups for one launch");
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid, (unsigned)grid_y), dim3(threads), 0, static_cast<hipStream_t>(stream), a);
   HIP_TRY(hipGetLastError());
+  return THA4_OK;
+}
+
+// kernels that work on rows, `per` of them a workgroup
+template <class K, class A>
+int launch_rows(K kernel, int per, int threads, A a, void* stream) {
+  const int64_t step = most_workgroups(threads) * per;
+  for (a.first = 0; a.first < a.rows; a.first += step) {
+    const int st = launch(kernel, ceil_div(std::min(a.rows - a.first, step), per), 1, threads, a, stream);
+    if (st != THA4_OK) return st;
+  }
   return THA4_OK;
 }
 
@@ -52,12 +66,12 @@ int launch(K kernel, int64_t grid, int64_t grid_y, int threads, const A& a, void
 template <class T>
 int quantize(const QuantArgs& a, void* stream) {
   if (a.cols % 8 || !aligned(a.x, a.x_stride, sizeof(T)) || reinterpret_cast<uintptr_t>(a.q) % 8 || a.q_stride % 8 || a.cols > 16384)
-    return launch(quantize_any_kernel<T>, a.rows, 1, 256, a, stream);
-  if (a.cols <= 512) return launch(quantize_kernel<T, 64, 1>, ceil_div(a.rows, 4), 1, 256, a, stream);
-  if (a.cols <= 2048) return launch(quantize_kernel<T, 256, 1>, a.rows, 1, 256, a, stream);
-  if (a.cols <= 4096) return launch(quantize_kernel<T, 256, 2>, a.rows, 1, 256, a, stream);
-  if (a.cols <= 8192) return launch(quantize_kernel<T, 256, 4>, a.rows, 1, 256, a, stream);
-  return launch(quantize_kernel<T, 1024, 2>, a.rows, 1, 1024, a, stream);
+    return launch_rows(quantize_any_kernel<T>, 1, 256, a, stream);
+  if (a.cols <= 512) return launch_rows(quantize_kernel<T, 64, 1>, 4, 256, a, stream);
+  if (a.cols <= 2048) return launch_rows(quantize_kernel<T, 256, 1>, 1, 256, a, stream);
+  if (a.cols <= 4096) return launch_rows(quantize_kernel<T, 256, 2>, 1, 256, a, stream);
+  if (a.cols <= 8192) return launch_rows(quantize_kernel<T, 256, 4>, 1, 256, a, stream);
+  return launch_rows(quantize_kernel<T, 1024, 2>, 1, 1024, a, stream);
 }
 
 // ---- product ----
@@ -73,18 +87,48 @@ const char* check_linear(const tha4_linear_i8_args& g) {
 bool inline_tokens(const tha4_linear_i8_args& g) { return g.m <= kInlineTokens && g.m * g.k <= kInlineBytes; }
 int64_t token_stride(const tha4_linear_i8_args& g) { return ceil_div(g.k, 16) * 16; }
 
+// m tokens from m0 on, n channels from n0 on
+LinearArgs part_of(const LinearArgs& a, int64_t m0, int64_t m, int64_t n0, int64_t n) {
+  LinearArgs b = a;
+  if (m0) {                                                              // (int8 tokens: the forms for few tokens take them all)
+    b.x = static_cast<const int8_t*>(a.x) + m0 * a.x_stride;
+    b.xs += m0;
+  }
+  b.w += n0 * a.w_stride;
+  b.ws += n0;
+  if (b.bias) b.bias += n0;
+  b.y = static_cast<char*>(a.y) + (m0 * a.y_stride + n0) * size_of(a.y_dtype);
+  b.m = std::min(a.m - m0, m);
+  b.n = std::min(a.n - n0, n);
+  return b;
+}
+
 template <class XT, int NT, int MT, bool INLINE>
 int few(const LinearArgs& a, bool al, void* stream) {
-  const int64_t nb = ceil_div(a.n, 16 * NT), mb = ceil_div(a.m, 16 * MT);
-  if constexpr (NT == 1)
-    if (!al) return launch(linear_few_kernel<XT, NT, MT, false, INLINE>, nb, mb, 512, a, stream);
-  return launch(linear_few_kernel<XT, NT, MT, true, INLINE>, nb, mb, 512, a, stream);
+  const int64_t step = most_workgroups(512) * 16 * NT, mb = ceil_div(a.m, 16 * MT);
+  for (int64_t n0 = 0; n0 < a.n; n0 += step) {
+    const LinearArgs b = part_of(a, 0, a.m, n0, step);
+    const int64_t nb = ceil_div(b.n, 16 * NT);
+    int st = THA4_OK;
+    if constexpr (NT == 1) st = al ? launch(linear_few_kernel<XT, NT, MT, true, INLINE>, nb, mb, 512, b, stream) : launch(linear_few_kernel<XT, NT, MT, false, INLINE>, nb, mb, 512, b, stream);
+    else st = launch(linear_few_kernel<XT, NT, MT, true, INLINE>, nb, mb, 512, b, stream);
+    if (st != THA4_OK) return st;
+  }
+  return THA4_OK;
 }
 template <int BM, int BN, int WM, int WN, int G, int STAGES>
 int tile(const LinearArgs& a, bool al, void* stream) {
-  const int64_t tiles = ceil_div(a.m, BM) * ceil_div(a.n, BN);
-  return al ? launch(linear_tile_kernel<BM, BN, 128, WM, WN, G, STAGES, true>, tiles, 1, 64 * WM * WN * G, a, stream)
-            : launch(linear_tile_kernel<BM, BN, 128, WM, WN, G, STAGES, false>, tiles, 1, 64 * WM * WN * G, a, stream);
+  constexpr int threads = 64 * WM * WN * G;
+  const int64_t most = most_workgroups(threads), step_n = most * BN, step_m = most / std::min(ceil_div(a.n, BN), most) * BM;
+  for (int64_t n0 = 0; n0 < a.n; n0 += step_n)
+    for (int64_t m0 = 0; m0 < a.m; m0 += step_m) {
+      const LinearArgs b = part_of(a, m0, step_m, n0, step_n);
+      const int64_t tiles = ceil_div(b.m, BM) * ceil_div(b.n, BN);
+      const int st = al ? launch(linear_tile_kernel<BM, BN, 128, WM, WN, G, STAGES, true>, tiles, 1, threads, b, stream)
+                        : launch(linear_tile_kernel<BM, BN, 128, WM, WN, G, STAGES, false>, tiles, 1, threads, b, stream);
+      if (st != THA4_OK) return st;
+    }
+  return THA4_OK;
 }
 // Which kernel: by the number of tokens, then the largest tile whose grid still covers most of the 256 CUs (us, w one of three in turn, bf16 out):
 //   m <= 32  weights straight into operands, wide tiles of channels where they fill the GPU:  32 x 16384 x 4096: 30.9 (NT 1), 20.3 (2), 17.2 (4);  32 x 8192 x 8192: 26.9, 21.9, 25.3
@@ -103,13 +147,13 @@ int product(const LinearArgs& a, bool al, void* stream) {
 // ---- norms ----
 template <class T, class R>
 int norm(const NormArgs& a, bool vector, void* stream) {
-  if (!vector || a.cols > 16384) return launch(residual_norm_any_kernel<T, R>, a.rows, 1, 256, a, stream);
-  if (a.cols <= 512) return launch(residual_norm_kernel<T, R, 64, 1>, ceil_div(a.rows, 4), 1, 256, a, stream);
-  if (a.cols <= 1024) return launch(residual_norm_kernel<T, R, 64, 2>, ceil_div(a.rows, 4), 1, 256, a, stream);
-  if (a.cols <= 2048) return launch(residual_norm_kernel<T, R, 256, 1>, a.rows, 1, 256, a, stream);
-  if (a.cols <= 4096) return launch(residual_norm_kernel<T, R, 256, 2>, a.rows, 1, 256, a, stream);
-  if (a.cols <= 8192) return launch(residual_norm_kernel<T, R, 512, 2>, a.rows, 1, 512, a, stream);
-  return launch(residual_norm_kernel<T, R, 1024, 2>, a.rows, 1, 1024, a, stream);
+  if (!vector || a.cols > 16384) return launch_rows(residual_norm_any_kernel<T, R>, 1, 256, a, stream);
+  if (a.cols <= 512) return launch_rows(residual_norm_kernel<T, R, 64, 1>, 4, 256, a, stream);
+  if (a.cols <= 1024) return launch_rows(residual_norm_kernel<T, R, 64, 2>, 4, 256, a, stream);
+  if (a.cols <= 2048) return launch_rows(residual_norm_kernel<T, R, 256, 1>, 1, 256, a, stream);
+  if (a.cols <= 4096) return launch_rows(residual_norm_kernel<T, R, 256, 2>, 1, 256, a, stream);
+  if (a.cols <= 8192) return launch_rows(residual_norm_kernel<T, R, 512, 2>, 1, 512, a, stream);
+  return launch_rows(residual_norm_kernel<T, R, 1024, 2>, 1, 1024, a, stream);
 }
 
 // ---- attention ----
@@ -157,12 +201,11 @@ const char* check_shape(const tha4_diff_attention_args& a) {
 }
 
 template <class T, int D>
-int attention(AttnArgs& a, const Plan& p, void* stream) {
+int attention_launch(const AttnArgs& a, const Plan& p, bool narrow, void* stream) {
   if (!p.few) {
     const int64_t heads = (int64_t)a.batch * a.heads;
-    // d = 32: workgroups of 64 queries where those of 128 leave CUs without one (8 frames of 256 tokens: 10.5 us against 13.4; at d = 64 the wider ones are as fast or faster)
     if constexpr (D == 32)
-      if (heads * ceil_div(a.q_len, 128) < 256) return launch(diff_prompt_kernel<T, D, 2>, heads * ceil_div(a.q_len, 64), 1, 256, a, stream);
+      if (narrow) return launch(diff_prompt_kernel<T, D, 2>, heads * ceil_div(a.q_len, 64), 1, 256, a, stream);
     return launch(diff_prompt_kernel<T, D, 4>, heads * ceil_div(a.q_len, 128), 1, 512, a, stream);
   }
   const int64_t tiles = (int64_t)a.batch * a.kv_heads * p.row_tiles;
@@ -170,8 +213,32 @@ int attention(AttnArgs& a, const Plan& p, void* stream) {
   if (st != THA4_OK || p.splits == 1) return st;
   return launch(diff_join_kernel<T, D>, tiles * p.part_rows, 1, 512, a, stream);
 }
+template <class T, int D>
+int attention(const AttnArgs& a, const Plan& p, void* stream) {
+  // d = 32: workgroups of 64 queries where those of 128 leave CUs without one (8 frames of 256 tokens: 10.5 us against 13.4; at d = 64 the wider ones are as fast or faster)
+  const bool narrow = D == 32 && (int64_t)a.batch * a.heads * ceil_div(a.q_len, 128) < 256;
+  // sequences of one launch: by the kernel that has the most threads for each
+  const int64_t tiles = (int64_t)a.kv_heads * p.row_tiles;
+  const int64_t threads = !p.few ? 512 * (a.heads * ceil_div(a.q_len, 128)) : std::max<int64_t>(256 * tiles * p.splits, p.splits == 1 ? 0 : 512 * tiles * p.part_rows);
+  const int64_t step = std::max<int64_t>(0xffffffffLL / std::max<int64_t>(threads, 1), 1);
+  for (int64_t b0 = 0; b0 < a.batch; b0 += step) {
+    AttnArgs c = a;
+    c.batch = (int32_t)std::min<int64_t>(a.batch - b0, step);
+    c.q = static_cast<const T*>(a.q) + b0 * a.qs[0];
+    c.k = static_cast<const T*>(a.k) + b0 * a.ks[0];
+    c.v = static_cast<const T*>(a.v) + b0 * a.vs[0];
+    c.out = static_cast<T*>(a.out) + b0 * a.os[0];
+    if (a.mask) c.mask = a.mask + b0 * a.ms[0];
+    if (a.q_lengths) c.q_lengths = a.q_lengths + b0;
+    if (a.kv_lengths) c.kv_lengths = a.kv_lengths + b0;
+    if (a.work) c.work = a.work + b0 * tiles * p.part_rows * p.splits * part_floats(D);
+    const int st = attention_launch<T, D>(c, p, narrow, stream);
+    if (st != THA4_OK) return st;
+  }
+  return THA4_OK;
+}
 template <class T>
-int attention(AttnArgs& a, int d, const Plan& p, void* stream) {
+int attention(const AttnArgs& a, int d, const Plan& p, void* stream) {
   return d == 32 ? attention<T, 32>(a, p, stream) : d == 64 ? attention<T, 64>(a, p, stream) : attention<T, 128>(a, p, stream);
 }
 
@@ -189,7 +256,7 @@ int tha4_quantize_tokens_i8(const void* x_dev, int x_dtype, int64_t rows, int64_
   const int dev = one_device({x_dev, q_dev, scale_dev});
   if (dev < 0) return bad("x / q / scale must be device pointers of one GPU");
   DeviceGuard guard(dev);
-  const QuantArgs a{x_dev, q_dev, scale_dev, rows, cols, x_row_stride, q_row_stride};
+  const QuantArgs a{x_dev, q_dev, scale_dev, rows, cols, x_row_stride, q_row_stride, 0};
   return x_dtype == THA4_F32 ? quantize<float>(a, stream) : x_dtype == THA4_F16 ? quantize<f16>(a, stream) : quantize<bf16>(a, stream);
 }
 
@@ -222,7 +289,7 @@ int tha4_linear_i8(const tha4_linear_i8_args* args, void* stream) {
     const int64_t stride = token_stride(g);
     int8_t* q = static_cast<int8_t*>(g.workspace_dev);
     float* scale = reinterpret_cast<float*>(q + g.m * stride);
-    const QuantArgs t{g.x_dev, q, scale, g.m, g.k, g.x_row_stride, stride};
+    const QuantArgs t{g.x_dev, q, scale, g.m, g.k, g.x_row_stride, stride, 0};
     const int st = g.x_dtype == THA4_F32 ? quantize<float>(t, stream) : g.x_dtype == THA4_F16 ? quantize<f16>(t, stream) : quantize<bf16>(t, stream);
     if (st != THA4_OK) return st;
     a.x = q;
@@ -258,7 +325,7 @@ int tha4_residual_norm(const tha4_residual_norm_args* args, void* stream) {
   DeviceGuard guard(dev);
   NormArgs a{g.residual_dev, g.branch_dev, g.gate_dev, g.residual_scale_vector_dev, g.post_weight_dev, g.post_bias_dev, g.pre_weight_dev, g.pre_bias_dev,
              g.film_scale_dev, g.film_shift_dev, g.h_dev, g.y_dev, g.rows, g.cols, g.residual_row_stride, g.branch_row_stride, g.gate_row_stride, g.film_row_stride,
-             g.h_row_stride, g.y_row_stride, g.gate_rows, g.film_rows, g.gate_dtype == THA4_F32, g.params_dtype == THA4_F32, g.post_norm, g.pre_norm,
+             g.h_row_stride, g.y_row_stride, g.gate_rows, g.film_rows, 0, g.gate_dtype == THA4_F32, g.params_dtype == THA4_F32, g.post_norm, g.pre_norm,
              g.gate_activation == THA4_GATE_SIGMOID, g.residual_scale, g.eps, 1.0f / (float)g.cols};
   const int64_t st = size_of(g.dtype), sr = size_of(g.residual_dtype), sg = size_of(g.gate_dtype), sp = size_of(g.params_dtype);
   const bool vector = g.cols % 8 == 0 && aligned(g.residual_dev, g.residual_row_stride, sr) && aligned(g.branch_dev, g.branch_row_stride, st) &&

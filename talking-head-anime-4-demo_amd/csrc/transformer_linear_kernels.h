@@ -14,6 +14,7 @@ struct QuantArgs {
   int8_t* q;
   float* scale;
   int64_t rows, cols, x_stride, q_stride;
+  int64_t first;               // row of the launch's first workgroup
 };
 
 struct MaxU32 { THA4_DEV float operator()(float a, float b) const {          // of bit patterns without sign: orders inf and NaN behind every number
@@ -62,7 +63,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) quantize_kernel(QuantAr
   constexpr int WAVES = TPR / 64, RPW = TPR < 256 ? 256 / TPR : 1;
   __shared__ float slots[RPW][WAVES];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
-  const int64_t row_ = (int64_t)blockIdx.x * RPW + sub;
+  const int64_t row_ = a.first + (int64_t)blockIdx.x * RPW + sub;
   const bool live = row_ < a.rows;
   const int64_t row = live ? row_ : a.rows - 1;
   const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
@@ -99,7 +100,7 @@ template <class T>
 __global__ void __launch_bounds__(256) quantize_any_kernel(QuantArgs a) {
   warm_kernarg<(int)sizeof(QuantArgs)>();
   __shared__ float slot[4];
-  const int64_t row = blockIdx.x;
+  const int64_t row = a.first + blockIdx.x;
   const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
   float m = 0.0f;
   for (int64_t c = threadIdx.x; c < a.cols; c += 256) m = MaxU32()(m, abs_bits((float)x[c]));

@@ -14,6 +14,7 @@ struct NormArgs {
   int64_t rows, cols;
   int64_t residual_stride, branch_stride, gate_stride, film_stride, h_stride, y_stride;
   int64_t gate_rows, film_rows;
+  int64_t first;               // row of the launch's first workgroup
   int32_t gate_f32, params_f32, post_norm, pre_norm, sigmoid;
   float residual_scale, eps, inv_cols;
 };
@@ -31,7 +32,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) residual_norm_kernel(No
   constexpr int WAVES = TPR / 64, RPW = TPR < 256 ? 256 / TPR : 1;
   __shared__ float slots[4][RPW][WAVES];
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR, wave = t / 64;
-  const int64_t row_ = (int64_t)blockIdx.x * RPW + sub;
+  const int64_t row_ = a.first + (int64_t)blockIdx.x * RPW + sub;
   const bool live = row_ < a.rows;                       // a row behind the last: the same work on the last row, no stores (the barriers stay uniform)
   const int64_t row = live ? row_ : a.rows - 1;
   const T* branch = static_cast<const T*>(a.branch) + row * a.branch_stride;
@@ -183,7 +184,7 @@ template <class T, class R>
 __global__ void __launch_bounds__(256) residual_norm_any_kernel(NormArgs a) {
   warm_kernarg<(int)sizeof(NormArgs)>();
   __shared__ float slots[4][4];
-  const int64_t row = blockIdx.x;
+  const int64_t row = a.first + blockIdx.x;
   const int t = threadIdx.x, wave = t / 64;
   const T* branch = static_cast<const T*>(a.branch) + row * a.branch_stride;
   const R* residual = static_cast<const R*>(a.residual) + row * a.residual_stride;

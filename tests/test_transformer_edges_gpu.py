@@ -195,3 +195,87 @@ def test_the_longest_sums_are_exact(m, n, k):
     one = lambda c: torch.ones(c, device="cuda:0")
     got = transformer.int8_linear(x, w, one(n), x_scale=one(m), out_dtype=F32)
     assert torch.equal(got, (x.double() @ w.double().t()).float())
+
+
+# ---- more rows, channels or sequences than one launch has workgroups -------------------------------------------------------------------------
+def places(n, *borders):
+    """Slices around 0, the borders between launches, and the end."""
+    return [slice(max(at - 40, 0), min(at + 40, n)) for at in (0, *borders, n)]
+
+
+@pytest.mark.parametrize("rows,cols", [(2 ** 24 + 333, 7), (2 ** 26 + 111, 8)])      # a workgroup a row, four rows a workgroup
+def test_more_rows_than_one_launch_holds(rows, cols):
+    g = rng(cols)
+    border = (2 ** 32 - 1) // 256 * (1 if cols == 7 else 4)
+    assert rows > border
+    x = torch.empty(rows, cols, dtype=BF16, device="cuda:0").normal_(generator=g)
+    q, s = transformer.quantize_tokens(x)
+    h, y = transformer.residual_norm(x, x, gate=x, pre_norm="layer")
+    for p in places(rows, border):
+        wq, ws = oracle.quantize(x[p])
+        assert torch.equal(q[p], wq) and torch.equal(s[p], ws)
+        (wh, bh), (wy, by) = oracle.residual_norm(x[p], x[p], x[p], pre_norm="layer")
+        within(h[p], (wh, bh))
+        within(y[p], (wy, by))
+    gate = randn(g, 1, cols, dtype=BF16)
+    film = randn(g, 1, cols), randn(g, 1, cols)
+    h, y = transformer.residual_norm(x, x, gate=gate, film=film)
+    for p in places(rows, border):
+        (wh, bh), (wy, by) = oracle.residual_norm(x[p], x[p], gate, film=film)
+        within(h[p], (wh, bh))
+        within(y[p], (wy, by))
+
+
+def test_more_channels_than_one_launch_holds():
+    n, k = 2 ** 27 + 1000, 3
+    g = rng(5)
+    border = (2 ** 32 - 1) // 512 * 16
+    w = torch.randint(-127, 128, (n, k), dtype=torch.int8, device="cuda:0", generator=g)
+    ws = torch.empty(n, device="cuda:0").uniform_(0.5, 2.0, generator=g)
+    bias = torch.empty(n, device="cuda:0").normal_(generator=g)
+    x = randn(g, 2, k, dtype=F16)
+    y = transformer.int8_linear(x, w, ws, bias=bias)
+    xq, xs = oracle.quantize(x)
+    y8 = transformer.int8_linear(xq[:1], w, ws, x_scale=xs[:1], bias=bias, out_dtype=BF16)
+    for p in places(n, border):
+        within(y[:, p], oracle.int8_linear(xq, xs, w[p], ws[p], bias[p], F16))
+        within(y8[:, p], oracle.int8_linear(xq[:1], xs[:1], w[p], ws[p], bias[p], BF16))
+
+
+def test_more_tiles_than_one_launch_holds():
+    m, k = 2 ** 31 - 1, 1
+    border = (2 ** 32 - 1) // 512 * 256
+    x = torch.arange(97, device="cuda:0", dtype=torch.int16).sub_(48).to(torch.int8).repeat(m // 97 + 1)[:m, None]
+    w = torch.tensor([[3]], dtype=torch.int8, device="cuda:0")
+    xs = torch.full((1,), 0.5, device="cuda:0").expand(m).contiguous()
+    y = transformer.int8_linear(x, w, torch.ones(1, device="cuda:0"), x_scale=xs, out_dtype=F16)
+    for p in places(m, border):
+        assert torch.equal(y[p], (x[p].float() * 1.5).half())
+
+
+@pytest.mark.parametrize("q_len,heads,batch", [(1, 1, 2 ** 24 + 100), (16, 1, 2 ** 24 + 100), (17, 2, 2 ** 22 + 100)])     # few queries in one range, prompts
+def test_more_sequences_than_one_launch_holds(q_len, heads, batch):
+    d = 32
+    g = rng(q_len)
+    border = (2 ** 32 - 1) // 256 if q_len <= 16 else (2 ** 32 - 1) // 512 // heads
+    q1, k1, v1, _, _ = attention_inputs(g, 7, q_len, 2, heads, 1, d, BF16)
+    lam = torch.zeros(4, d, device="cuda:0")
+    index = torch.arange(batch, device="cuda:0") % 7
+    q = q1[:1].expand(batch, -1, -1, -1)
+    v = v1[index]
+    k = k1[:1].expand(batch, -1, -1, -1)
+    lengths = (index % 3).to(torch.int32)
+    mask = (torch.arange(batch, device="cuda:0") % 5 != 3)[:, None, None, None]
+    got = transformer.differential_attention(q, k, v, lam, 0.5, kv_lengths=lengths, mask=mask, norm=False)
+    for p in places(batch, border):
+        kw = dict(kv_lengths=lengths[p], mask=mask[p], norm=False)
+        within(got[p], oracle.differential_attention(q[p], k[p], v[p], lam, 0.5, **kw))
+    del got
+    q_lengths = (torch.arange(batch, device="cuda:0") % (q_len + 1)).to(torch.int32)
+    out = torch.empty(batch, q_len, heads, 2 * d, dtype=BF16, device="cuda:0").fill_(7.0)
+    transformer.differential_attention(q, k, v, lam, 0.5, q_lengths=q_lengths, causal=True, norm=False, out=out)
+    for p in places(batch, border):
+        want, bound = oracle.differential_attention(q[p], k[p], v[p], lam, 0.5, q_lengths=q_lengths[p], causal=True, norm=False)
+        valid = torch.arange(q_len, device="cuda:0")[None] < q_lengths[p][:, None]
+        assert (out[p][~valid] == 7.0).all()
+        within(out[p][valid], (want[valid], bound[valid]))
