@@ -19,6 +19,7 @@ using namespace tha4::xf;
 namespace {
 
 constexpr int64_t kMaxGrid = 0x7fffffff;
+constexpr float kLog2e = 1.44269504088896340736f;
 
 int64_t size_of(int dtype) { return dtype == THA4_F32 ? 4 : 2; }
 bool known(int dtype) { return dtype == THA4_F32 || dtype == THA4_F16 || dtype == THA4_BF16; }
@@ -349,7 +350,7 @@ int tha4_diff_attention(const tha4_diff_attention_args* args, void* stream) {
   if (!args) return bad("args must not be NULL");
   const tha4_diff_attention_args& g = *args;
   if (const char* e = check_shape(g)) return bad(e);
-  if (!(g.scale > 0.0f) || !std::isfinite(g.scale)) return bad("scale must be positive and finite");
+  if (!(g.scale > 0.0f) || !std::isfinite(g.scale * kLog2e)) return bad("scale must be positive and finite, times log2(e) too");
   if (!(g.eps >= 0.0f) || !std::isfinite(g.lambda_init)) return bad("eps must not be negative and lambda_init must be finite");
   if (g.batch == 0 || g.q_len == 0) return THA4_OK;
   if (!g.q_dev || !g.out_dev || !g.lambda_vectors_dev) return bad("q / out / lambda_vectors must not be NULL");
@@ -384,7 +385,7 @@ int tha4_diff_attention(const tha4_diff_attention_args* args, void* stream) {
   a.batch = g.batch; a.q_len = g.q_len; a.k_len = g.k_len; a.heads = g.heads; a.kv_heads = g.kv_heads; a.group = g.heads / g.kv_heads;
   a.causal = g.causal; a.norm = g.norm;
   a.row_tiles = p.row_tiles; a.splits = p.splits; a.chunk = p.chunk; a.part_rows = p.part_rows;
-  a.c = g.scale * 1.44269504088896340736f; a.slack = (g.dtype == THA4_F16 ? Mat<f16>::SLACK : Mat<bf16>::SLACK) / a.c; a.lambda_init = g.lambda_init; a.eps = g.eps;
+  a.c = g.scale * kLog2e; a.slack = (g.dtype == THA4_F16 ? Mat<f16>::SLACK : Mat<bf16>::SLACK) / a.c; a.lambda_init = g.lambda_init; a.eps = g.eps;
   return g.dtype == THA4_F16 ? attention<f16>(a, g.head_dim, p, stream) : attention<bf16>(a, g.head_dim, p, stream);
 }
 

@@ -241,3 +241,11 @@ def test_oracle_attention_of_nothing_is_zero_without_eps():
     out, bound = oracle.differential_attention(q, k, v, torch.zeros(4, 32), 0.5, kv_lengths=torch.tensor([0, 6]), eps=0.0)
     assert not out[0].any() and out[1].abs().min(-1)[0].isfinite().all() and bound.isfinite().all()
     assert torch.allclose((out[1] ** 2).mean(-1), torch.full((4, 1), 0.25, dtype=torch.float64))
+
+
+def test_attention_refuses_a_scale_that_overflows_with_its_factor(lib):
+    """The softmax is taken in powers of two: scale * log2(e) has to be a number, or every difference of scores is 0 * inf."""
+    p, keep = host(256)
+    p = C.c_void_p((p.value + 15) // 16 * 16)
+    refused(lib, lib.tha4_diff_attention(attention_args(p, scale=2.5e38), None), "scale")
+    refused(lib, lib.tha4_diff_attention(attention_args(p, scale=2.3e38), None), "device pointers")
