@@ -2,6 +2,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <cstdio>
 #include <string>
 
 #include "tha4_hip.h"
@@ -12,11 +13,17 @@ namespace tha4 {
 __attribute__((visibility("hidden"))) int fail(int code, const char* msg) noexcept;
 inline int fail(int code, const std::string& msg) { return fail(code, msg.c_str()); }
 
+// (no allocation: nothing may be thrown through a C entry point)
+inline int fail_hip(const char* expr, hipError_t e) noexcept {
+  char text[512];
+  snprintf(text, sizeof(text), "%s: %s", expr, hipGetErrorString(e));
+  return fail(THA4_ERR_HIP, text);
+}
+
 #define HIP_TRY(expr)                                                                              \
   do {                                                                                             \
     hipError_t e_ = (expr);                                                                        \
-    if (e_ != hipSuccess)                                                                          \
-      return fail(THA4_ERR_HIP, std::string(#expr) + ": " + hipGetErrorString(e_));                \
+    if (e_ != hipSuccess) return fail_hip(#expr, e_);                                              \
   } while (0)
 
 struct DeviceGuard {

@@ -6,7 +6,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <string>
 
 #include "tha4_host.h"
 #include "transformer_attention_kernels.h"

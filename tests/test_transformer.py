@@ -249,3 +249,16 @@ def test_attention_refuses_a_scale_that_overflows_with_its_factor(lib):
     p = C.c_void_p((p.value + 15) // 16 * 16)
     refused(lib, lib.tha4_diff_attention(attention_args(p, scale=2.5e38), None), "scale")
     refused(lib, lib.tha4_diff_attention(attention_args(p, scale=2.3e38), None), "device pointers")
+
+
+def test_nothing_in_the_operators_object_can_throw(built):
+    """Host code of the operators allocates nothing and throws nothing (a C entry point has no one to catch it): its object needs no symbol for either."""
+    import os
+    import subprocess
+    from tha4_amd import _build
+    obj = os.path.join(_build.OBJECTS, "tha4_transformer.product.o")
+    if not os.path.exists(obj):
+        pytest.skip("the library was built elsewhere: its objects are not here")
+    names = subprocess.run(["nm", "-u", "-C", obj], capture_output=True, text=True, check=True).stdout
+    for word in ("std::__throw", "__cxa_throw", "operator new", "basic_string", "vector"):
+        assert word not in names, [l for l in names.splitlines() if word in l]
