@@ -364,7 +364,7 @@ int tha4_residual_norm(const tha4_residual_norm_args* args, void* stream);
  * (lambda_vectors [4][heads or 1][head_dim] fp32, in fp32), then, with `norm` non-zero, (1 - lambda_init) * o / sqrt(mean(o^2) + eps) * norm_weight.
  *   q [batch][q_len][2 heads][d], k [batch][k_len][2 kv_heads][d]: heads 2h and 2h + 1 are the pair of head h;  v [batch][k_len][kv_heads][2d];
  *   out [batch][q_len][heads][2d];  d = 32, 64 or 128;  heads a multiple of kv_heads;  dtype f16 or bf16; rows contiguous and 16-byte aligned;
- *   strides in elements over (batch, token, head), token strides of k and v below 2^24.
+ *   strides in elements over (batch, token, head), token strides of k and v below 2^24; rows of out must not overlap each other, q, k or v.
  * kv_lengths [batch] (NULL: k_len): keys at or behind it are never read into a result, whatever they hold.  q_lengths [batch] (NULL: q_len): query rows at or behind it are
  * not written.  Lengths outside [0, k_len] / [0, q_len] count as the nearer end.  causal: query i sees key j <= i + kv_length - q_length (the last
  * query the last key).  mask (NULL: none): bytes, non-zero = visible, over (batch, head, query, key) with strides in bytes (0 = broadcast).

@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <utility>
 
 #include "tha4_host.h"
 #include "transformer_attention_kernels.h"
@@ -200,6 +201,23 @@ const char* check_shape(const tha4_diff_attention_args& a) {
   return nullptr;
 }
 
+// whether the rows of `out` that (batch, token, head) address share elements: every stride has to step over what the smaller ones span
+bool overlaps_itself(const tha4_diff_attention_args& g) {
+  int64_t n[3] = {g.batch, g.q_len, g.heads}, s[3] = {g.out_stride[0], g.out_stride[1], g.out_stride[2]}, span = 2 * g.head_dim;
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 2 - i; ++j)
+      if (s[j] > s[j + 1]) {
+        std::swap(s[j], s[j + 1]);
+        std::swap(n[j], n[j + 1]);
+      }
+  for (int i = 0; i < 3; ++i) {
+    if (n[i] == 1) continue;
+    if (s[i] < span) return true;
+    span += s[i] * (n[i] - 1);
+  }
+  return false;
+}
+
 template <class T, int D>
 int attention_launch(const AttnArgs& a, const Plan& p, bool narrow, void* stream) {
   if (!p.few) {
@@ -364,6 +382,7 @@ int tha4_diff_attention(const tha4_diff_attention_args* args, void* stream) {
   for (int i = 0; i < 4; ++i)
     if (g.mask_dev && g.mask_stride[i] < 0) return bad("strides must not be negative");
   if (g.lambda_vector_stride < 0 || g.lambda_head_stride < 0) return bad("strides must not be negative");
+  if (overlaps_itself(g)) return bad("rows of out overlap each other");
   const Plan p = plan_of(g);
   const int64_t need = tha4_diff_attention_workspace(args);
   if (need && (!g.workspace_dev || g.workspace_bytes < need || reinterpret_cast<uintptr_t>(g.workspace_dev) % 16))

@@ -253,7 +253,7 @@ def differential_attention(q: Tensor, k: Tensor, v: Tensor, lambda_vectors: Tens
     cache).  lambda_vectors fp32 [4, d] or [4, heads, d].  scale: 1 / sqrt(d).
 
     kv_lengths int32 [batch]: the valid keys of each sequence (what lies behind them is never read into a result); q_lengths int32 [batch]: its valid queries - rows
-    behind them are zero, or left as they are in a given ``out``.  causal: the last valid query sees the last valid key.  mask: bool, broadcastable to
+    behind them are zero, or left as they are in a given ``out`` (which shares no memory with q, k or v).  causal: the last valid query sees the last valid key.  mask: bool, broadcastable to
     [batch, heads, q_len, k_len], True = visible.  A query that sees no key answers zero.  k_len may be 0."""
     lib = _library()
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:

@@ -262,3 +262,14 @@ def test_nothing_in_the_operators_object_can_throw(built):
     names = subprocess.run(["nm", "-u", "-C", obj], capture_output=True, text=True, check=True).stdout
     for word in ("std::__throw", "__cxa_throw", "operator new", "basic_string", "vector"):
         assert word not in names, [l for l in names.splitlines() if word in l]
+
+
+def test_attention_refuses_an_output_whose_rows_overlap(lib):
+    p, keep = host(256)
+    p = C.c_void_p((p.value + 15) // 16 * 16)
+    shape = dict(batch=2, q_len=3, heads=4, kv_heads=2, k_len=5, head_dim=32)
+    for batch, token, head in ((0, 256, 64), (768, 0, 64), (768, 256, 0), (768, 256, 60), (768, 128, 64), (512, 256, 64), (64, 512, 64)):
+        refused(lib, lib.tha4_diff_attention(attention_args(p, out_stride_0=batch, out_stride_1=token, out_stride_2=head, **shape), None), "overlap")
+    for batch, token, head in ((768, 256, 64), (256, 512, 64), (64 * 12, 64, 64 * 3), (64, 512, 128), (64 * 3, 64, 64 * 6), (0, 256, 64)):
+        many = dict(shape, batch=1) if batch == 0 else shape                      # (64, 512, 128): rows b + 8 t + 2 h, all different
+        refused(lib, lib.tha4_diff_attention(attention_args(p, out_stride_0=batch, out_stride_1=token, out_stride_2=head, **many), None), "device pointers")
