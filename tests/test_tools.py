@@ -41,3 +41,16 @@ def test_variants_are_built_from_every_source(tool, more, commands, monkeypatch)
     assert builds
     for c in builds:
         assert {os.path.basename(a) for a in c if a.endswith(".hip")} == set(_build.SOURCES)
+
+
+def test_build_compiles_every_piece_whenever_it_is_called(monkeypatch):
+    """A library that is there already says nothing about the sources that are there now."""
+    import torch  # noqa: F401  (loaded before ctypes is replaced)
+    import __graft_entry__ as entry
+    asked = []
+    for module, names in ((_build, ("build_native", "build_forced_wait_twin")), (entry, ("build_emulator", "build_emulator_full", "build_ops_device"))):
+        for name in names:
+            monkeypatch.setattr(module, name, lambda force=False, name=name: asked.append((name, force)) or _build.LIB)
+    monkeypatch.setattr("ctypes.CDLL", lambda path: type("Lib", (), {"__getattr__": lambda self, n: n})())
+    entry.build()
+    assert sorted(asked) == sorted((n, True) for n in ("build_native", "build_forced_wait_twin", "build_emulator", "build_emulator_full", "build_ops_device"))
