@@ -91,8 +91,9 @@ def residual_norm(residual, branch=None, gate=None, gate_activation="none", resi
         y = y * (1 + s) + t
     out = residual.dtype
     ydt = residual.dtype if branch is None else branch.dtype
-    return ((h.reshape(shape), (dh + half(out) * (h.abs() + dh) + 1e-30).reshape(shape)),
-            (y.reshape(shape), (dy + half(ydt) * (y.abs() + dy) + 1e-30).reshape(shape)))
+    # (below the smallest normal number a rounding is off by half a step there, however small the value: smallest_normal * half)
+    return ((h.reshape(shape), (dh + half(out) * (h.abs() + dh) + torch.finfo(out).smallest_normal * half(out)).reshape(shape)),
+            (y.reshape(shape), (dy + half(ydt) * (y.abs() + dy) + torch.finfo(ydt).smallest_normal * half(ydt)).reshape(shape)))
 
 
 def visible(batch, q_len, k_len, causal, q_lengths, kv_lengths, mask, device):

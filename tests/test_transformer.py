@@ -273,3 +273,11 @@ def test_attention_refuses_an_output_whose_rows_overlap(lib):
     for batch, token, head in ((768, 256, 64), (256, 512, 64), (64 * 12, 64, 64 * 3), (64, 512, 128), (64 * 3, 64, 64 * 6), (0, 256, 64)):
         many = dict(shape, batch=1) if batch == 0 else shape                      # (64, 512, 128): rows b + 8 t + 2 h, all different
         refused(lib, lib.tha4_diff_attention(attention_args(p, out_stride_0=batch, out_stride_1=token, out_stride_2=head, **many), None), "device pointers")
+
+
+def test_oracle_norm_bound_holds_for_a_perfect_answer_among_the_subnormals():
+    """The least that an fp16 answer can be off, for values down to the subnormals, is inside the bound."""
+    x = (torch.randn(4, 64, generator=torch.Generator().manual_seed(4)) * torch.logspace(-7, 0, 64)).half()
+    for want, bound in oracle.residual_norm(x, x, post_norm="none", pre_norm="rms", eps=1.0):
+        assert ((want.half().double() - want).abs() <= bound).all()
+        assert (want.abs() < 2.0 ** -14).any()
