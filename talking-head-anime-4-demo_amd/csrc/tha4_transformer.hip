@@ -233,7 +233,7 @@ int attention_launch(const AttnArgs& a, const Plan& p, bool narrow, void* stream
 }
 template <class T, int D>
 int attention(const AttnArgs& a, const Plan& p, void* stream) {
-  // d = 32: workgroups of 64 queries where those of 128 leave CUs without one (8 frames of 256 tokens: 10.5 us against 13.4; at d = 64 the wider ones are as fast or faster)
+  // d = 32: workgroups of 64 queries where those of 128 leave CUs without one (8 frames of 256 tokens: 11.4 us against 15.7, in a graph; at d = 64 the wider ones are as fast or faster)
   const bool narrow = D == 32 && (int64_t)a.batch * a.heads * ceil_div(a.q_len, 128) < 256;
   // sequences of one launch: by the kernel that has the most threads for each
   const int64_t tiles = (int64_t)a.kv_heads * p.row_tiles;

@@ -10,8 +10,8 @@
 //
 // Precision: scores, maxima, sums, accumulators, lambda and the norm are fp32.  A weight p is an operand of the product with V as the sum of two numbers of the inputs' type, hi and p - hi: off by 2^-16 (bf16)
 // or 2^-22 (fp16) of itself, where one number would be off by 2^-8 or 2^-11 - which the difference of the maps and the norm behind it enlarge by |A1| + lambda |A2| over |A1 - lambda A2|: seven times what
-// the result's own rounding costs where the maps see nearly the same.  The second product of a pair costs nothing where memory or latency bounds (one token over a cache, 8 frames of 256 tokens) and 5 / 3 of the matrix work
-// elsewhere: 8192 x 8192, d = 128: 596 us instead of 412; d = 64, padded: 84 instead of 66.
+// the result's own rounding costs where the maps see nearly the same.  The second product of a pair costs nothing where the cache is the traffic (one token) and 5 / 3 of the matrix work
+// elsewhere: 8192 x 8192, d = 128: 588 us instead of 416; d = 64, padded: 78 instead of 61; 8 frames of 256 tokens, d = 32: the kernel 13.9 instead of 11.6, the call 11.9 instead of 11.7.
 #pragma once
 #include "transformer_types.h"
 
@@ -125,7 +125,8 @@ THA4_DEV float norm_factor(const AttnArgs& a, float ss) { return !a.norm ? 1.0f 
 //
 // Two waves share a SIMD: one of each map.  A group costs a wave a stretch of matrix products (with V of the group before, then with K of this one) and a stretch of
 // vector arithmetic (the softmax); the two waves run them in opposite phases, a barrier between the phases, so that one's arithmetic runs under the other's products.
-// Measured, causal: 8192 x 8192, 8 heads, d = 128: 607 us (in step, without the phases: 637): 680 TFLOP/s of the 12 d operations a pair that the formula has, 1130 of the 20 d that run.
+// Measured, causal: 8192 x 8192, 8 heads, d = 128: 588 - 607 us (in step, without the phases: 637): 700 TFLOP/s of the 12 d operations a pair that the formula has, 1170 of
+// the 20 d that run.
 template <int D>
 struct Tile {
   static constexpr int J = D == 128 ? 1 : 2, KEYS = 32 * J, SLOTS = 4;  // 32-key tiles of a group: one where the accumulator leaves no registers for two
@@ -340,7 +341,7 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
   };
 
   if constexpr (RG == 2) {
-    // Four waves, each alone on its SIMD (or beside another workgroup's): no partner to take turns with (8 frames of 256 tokens, d = 32: 10.5 us in step, 14.0 us in phases)
+    // Four waves, each alone on its SIMD (or beside another workgroup's): no partner to take turns with (8 frames of 256 tokens, d = 32, in a graph: 11.4 us in step, 13.7 us in phases)
 #pragma unroll
     for (int g = 0; g < 3; ++g) { request_k(g); request_v(g); }
     auto enter = [&](int g) {
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(128 * RG, 2) diff_prompt_kernel(AttnArgs a) {
 // A workgroup owns a range of the keys; its four waves take turns of 32 keys, each with running statistics and LDS of its own and without barriers.  The next turn's K is
 // requested as soon as this turn's has been read into operands, the next V behind the product with this one: a wave always has one of the two in flight,
 // asynchronously and straight into LDS, behind counted waits.  The waves meet in LDS, the ranges in a second launch.
-// Measured: 32 caches of up to 16384 keys, 16 heads on 4, d = 64 (544 MB): 115 us + 6.5 us for the join, 4.7 TB/s;  131072 keys, 8 heads on 2, d = 128 (268 MB): 50 + 8 us, 5.3 TB/s.
+// Measured: 32 caches of up to 16384 keys, 16 heads on 4, d = 64 (544 MB): 116 us + 6.5 us for the join, 4.7 TB/s;  131072 keys, 8 heads on 2, d = 128 (268 MB): 51 + 8 us, 5.3 TB/s.
 constexpr int kTurn = 32, kRows = 16, kMaxSplits = 512;
 
 template <int D>

@@ -1,5 +1,5 @@
-"""Operators of a transformer block over token sequences, at inference, on the GPU: what the posers' networks have inside (attention, normalisation +
-FiLM + residual, reduced-precision matrix products), for sequences of any length, prompts and single tokens over a cache.
+"""Operators of a transformer block over token sequences, at inference, on the GPU: relatives of what the posers' networks have inside (attention, normalisation +
+FiLM + residual, reduced-precision matrix products), for sequences of any length, prompts and single tokens over a cache.  The posers do not call them.
 
 ``quantize_tokens``         tokens (or weight rows) to int8 with one scale each
 ``int8_linear``             int8 x int8 matrix product with scales for each token and channel
