@@ -279,3 +279,73 @@ def test_more_sequences_than_one_launch_holds(q_len, heads, batch):
         valid = torch.arange(q_len, device="cuda:0")[None] < q_lengths[p][:, None]
         assert (out[p][~valid] == 7.0).all()
         within(out[p][valid], (want[valid], bound[valid]))
+
+
+# ---- graphs whose lengths and masks change between replays -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("q_len,k_len", [(300, 300), (3, 5000)])
+def test_a_captured_padded_batch_replays_with_other_lengths(q_len, k_len):
+    """Lengths, mask and inputs are read when the graph runs; rows behind the last query are zero again in every replay.  q has to be copied first (2-byte aligned)."""
+    g = rng(q_len)
+    q, k, v, lam, w = attention_inputs(g, 4, q_len, k_len, 4, 2, 64, F16)
+    q = torch.empty(q.numel() + 1, dtype=F16, device="cuda:0")[1:].view_as(q).copy_(q)
+    nq, nk = torch.zeros(4, dtype=torch.int32, device="cuda:0"), torch.zeros(4, dtype=torch.int32, device="cuda:0")
+    mask = torch.ones(4, 1, q_len, k_len, dtype=torch.bool, device="cuda:0")
+
+    def step():
+        return transformer.differential_attention(q, k, v, lam, 0.5, causal=True, q_lengths=nq, kv_lengths=nk, mask=mask, norm_weight=w)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for r in range(5):
+        nq.copy_(torch.randint(0, q_len + 1, (4,), device="cuda:0", generator=g))
+        nk.copy_(torch.randint(0, k_len + 1, (4,), device="cuda:0", generator=g))
+        mask.copy_(torch.rand(mask.shape, device="cuda:0", generator=g) > 0.3)
+        q.normal_(generator=g)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        within(out, oracle.differential_attention(q, k, v, lam, 0.5, causal=True, q_lengths=nq, kv_lengths=nk, mask=mask, norm_weight=w))
+
+
+def test_two_host_threads_call_at_once():
+    """Each on a stream of its own, with refused calls between: the bits of a call made alone, and every thread its own error text."""
+    import threading
+    g = rng(21)
+    q, k, v, lam, w = attention_inputs(g, 2, 2, 3000, 8, 2, 64, BF16)
+    x, wq, ws = randn(g, 7, 1024, dtype=F16), torch.randint(-127, 128, (512, 1024), device="cuda:0", generator=g).to(torch.int8), randn(g, 512).exp()
+
+    def calls():
+        return [transformer.differential_attention(q, k, v, lam, 0.5), transformer.int8_linear(x, wq, ws), *transformer.residual_norm(x, x)]
+
+    want = calls()
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(refused, word):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(30):
+                    got = calls()
+                    with pytest.raises(_capi.Tha4Error, match=word):
+                        refused()
+                    s.synchronize()
+                    assert all(torch.equal(a, b) for a, b in zip(got, want))
+        except BaseException as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=a) for a in ((lambda: transformer.residual_norm(x, x, eps=-1.0), "eps"),
+                                                               (lambda: transformer.differential_attention(q, k, v, lam, 0.5, scale=-1.0), "scale"))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
